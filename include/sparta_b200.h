@@ -243,6 +243,50 @@ int sparta_attn_fwd_gather(const void* Q, const void* K, const void* V, void* O,
                            int32_t* status, void* const* copies, int n_copies, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Dropout whose decisions come from a counter (Philox4x32 with seven rounds) and are never stored (no counterpart in
+ * the reference).  Position (batch b, row r, column c) of call number `call` is kept when the 16-bit value at place
+ * c % 8 of Philox(key = seed, counter = (c / 8, r, b, call)) is not below round(65536 p); kept values are scaled by
+ * 65536 / (65536 - round(65536 p)), the others are 0.  The decisions do not depend on the layout: a dense tensor,
+ * block values and the fused attention below drop the same positions.  The backward pass is the same call on the
+ * output's gradient.
+ *
+ * rng       device int64[2] (seed, call number; of the call number the lower 32 bits count) or NULL: then the
+ *           arguments `seed` and `call`.  A captured graph draws new numbers when `rng` is given and rewritten.
+ * sparta_dropout         x, y: [batch, H, W] dense, any sizes; y 16-byte aligned
+ * sparta_dropout_blocks  x, y: [batch, val_stride_blocks * BH * BW] in BCSR order, BW >= 8; values behind the last of
+ *                        the *nnz blocks are written 0
+ */
+int sparta_dropout(const void* x, void* y, int batch, int H, int W, double p, const int64_t* rng, uint64_t seed,
+                   uint64_t call, int dtype, void* stream);
+
+int sparta_dropout_blocks(const void* x, void* y, const int32_t* bcsr_idx, const int32_t* nnz, int batch, int BH, int BW,
+                          int64_t val_stride_blocks, double p, const int64_t* rng, uint64_t seed, uint64_t call,
+                          int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Rotary positions on one or two tensors (queries and keys) in one launch (no counterpart in the reference).
+ * y[b, h, i] = x[b, h, i] with each pair of its first rotary_dim elements turned by positions[b, i] * f_k and scaled by
+ * `magnitude`; pairs are (2 k, 2 k + 1) when interleaved, else (k, k + rotary_dim / 2).
+ *
+ * h_tensors    host array of `count` (1 or 2) records: x with element strides for batch, head and token (innermost
+ *              stride 1), y contiguous [batch, heads, n, dim], positions int32 or int64 [n], or [batch, n] with
+ *              positions_per_batch; NULL positions count 0, 1, 2 ...
+ * turns        device uint64 [rotary_dim / 2]: f_k / (2 pi) * 2^64, rounded, modulo 2^64
+ * backward     turns by the negative angle (x = gradient of the output, y = gradient of the input)
+ */
+typedef struct sparta_rotary_tensor {
+  const void* x;
+  void* y;
+  const void* positions;
+  int64_t stride_batch, stride_head, stride_token;
+  int32_t batch, heads, n;
+  int32_t positions_per_batch;
+} sparta_rotary_tensor;
+
+int sparta_rotary(const sparta_rotary_tensor* h_tensors, int count, const uint64_t* turns, int dim, int rotary_dim,
+                  int interleaved, float magnitude, int backward, int positions_are_64, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Tile table: what sparta.nn.tune searches over in the reference
  * (sparta/specializer/kernels/look_up_tables/sparta_matmul_lut.csv, sparta/nn/module_tuner.py:169)
  * becomes a fixed list of prebuilt kernels.  op: 0 sdd, 1 dsd, 2 dds, 3 softmax, 4 attention.

@@ -3,9 +3,10 @@
 There is no CPU or eager fallback: when the shared library is missing, ``lib()`` raises, and every
 operator of this package goes through ``lib()``.
 """
+import contextlib
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from typing import Optional
 
 import torch
@@ -43,6 +44,15 @@ class TileEntry(ctypes.Structure):
     ]
 
 
+class RotaryTensor(ctypes.Structure):
+    """Mirror of ``sparta_rotary_tensor``."""
+    _fields_ = [
+        ('x', c_void_p), ('y', c_void_p), ('positions', c_void_p),
+        ('stride_batch', c_int64), ('stride_head', c_int64), ('stride_token', c_int64),
+        ('batch', c_int32), ('heads', c_int32), ('n', c_int32), ('positions_per_batch', c_int32),
+    ]
+
+
 # name -> (restype, argtypes); the list is also what the symbol-export test walks
 SIGNATURES = {
     'sparta_version': (c_int, []),
@@ -76,6 +86,12 @@ SIGNATURES = {
     'sparta_attn_fwd_gather': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_float, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
                                        c_void_p, POINTER(c_void_p), c_int, c_void_p]),
+    'sparta_dropout': (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_double, c_void_p, c_uint64, c_uint64,
+                               c_int, c_void_p]),
+    'sparta_dropout_blocks': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int64,
+                                      c_double, c_void_p, c_uint64, c_uint64, c_int, c_void_p]),
+    'sparta_rotary': (c_int, [POINTER(RotaryTensor), c_int, c_void_p, c_int, c_int, c_int, c_float, c_int,
+                              c_int, c_int, c_void_p]),
     'sparta_last_status': (c_int, [POINTER(c_int32)]),
     'sparta_tile_table': (c_int, [c_int, c_int, POINTER(TileEntry), c_int]),
 }
@@ -114,6 +130,14 @@ def check(status: int, where: str):
 
 def stream_ptr(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is current; free of charge when it is already."""
+    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -1,3 +1,4 @@
 from sparta_b200.specializer.operators import (
-    OperatorBase, SparseLinear, SparseBatchMatMul, SparseSoftmax, SparseAttention,
+    OperatorBase, SparseLinear, SparseBatchMatMul, SparseSoftmax, SparseAttention, SparseDropout,
+    RotaryEmbedding,
 )
