@@ -214,7 +214,7 @@ int sparta_softmax_bwd(const void* dy, const void* y, void* dx, const int32_t* r
  * Replaces the three launches of SparseAttention.forward
  * (sparta/specializer/operators/sparse_attention.py:76-80): dds(Q,K^T) -> sparse softmax -> sdd(P,V);
  * the score tensor is never written to global memory.
- * Q: [heads, Nt, D]; K, V: [heads, Ns, D]; O: [heads, Nt, D]; fp16 or bf16; D in {64, 128}.
+ * Q: [heads, Nt, D]; K, V: [heads, Ns, D]; O: [heads, Nt, D]; fp16 or bf16; D in {64, 128}; Nt, Ns multiples of BLK.
  * row_ptr / bcsr_idx / nnz: BCSR of the [Nt, Ns] mask with BLK x BLK blocks (BLK = 64), shared by
  * every head.  mask: the dense uint8 [Nt, Ns] mask for element-level masking inside kept blocks, or
  * NULL when kept blocks are completely non-zero.  lse: optional fp32 [heads, Nt] log-sum-exp output.
@@ -241,6 +241,49 @@ int sparta_attn_fwd_gather(const void* Q, const void* K, const void* V, void* O,
                            const int32_t* bcsr_idx, const int32_t* nnz, const uint8_t* mask, float scale,
                            int heads, int Nt, int Ns, int D, int BLK, int dtype, float* lse,
                            int32_t* status, void* const* copies, int n_copies, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Training form of the fused attention: the forward pass that keeps the row log-sum-exp, and the backward pass that
+ * recomputes the probabilities from it (the reference trains through its three operators).  Both take dropout on the
+ * probabilities (sparta_dropout's decisions for a [heads, Nt, Ns] tensor) and key / value heads shared by
+ * heads / kv_heads consecutive query heads.  Gradients of shared heads are summed; every gradient is written once, in a
+ * fixed order of additions.
+ *   Q, O, dO, dQ: [heads, Nt, D]; K, V, dK, dV: [kv_heads, Ns, D]; fp16 / bf16; D in {64, 128}; Nt, Ns multiples of
+ *   BLK = 64, Ns <= 65536 (backward: Nt too).  row_ptr / bcsr_idx / mask as for sparta_attn_fwd; rows without any score
+ *   give O = 0 and dQ = 0.  lse: fp32 [heads, Nt], written by the forward pass (or NULL there) and read by the backward
+ *   pass, which needs the forward's O, mask, indexes and random numbers again.  dQ may be NULL, and so may dK and dV
+ *   together: what is not wanted is not computed.
+ *   dropout in [0, 1], rng / seed / call as for sparta_dropout.
+ *   workspace (backward only): sparta_attn_train_bwd_workspace_bytes(), 16-byte aligned, no initial contents.
+ */
+typedef struct sparta_attn_train_args {
+  const void* Q;
+  const void* K;
+  const void* V;
+  void* O;
+  float* lse;
+  const void* dO; /* backward only, like the next five */
+  void* dQ;
+  void* dK;
+  void* dV;
+  void* workspace;
+  size_t workspace_bytes;
+  const int32_t* row_ptr;
+  const int32_t* bcsr_idx;
+  const uint8_t* mask;
+  const int64_t* rng;
+  uint64_t seed, call;
+  int32_t* status;
+  double dropout;
+  float scale;
+  int32_t heads, kv_heads, Nt, Ns, D, BLK, dtype;
+} sparta_attn_train_args;
+
+int sparta_attn_train_fwd(const sparta_attn_train_args* h_args, void* stream);
+
+size_t sparta_attn_train_bwd_workspace_bytes(int heads, int Nt, int Ns);
+
+int sparta_attn_train_bwd(const sparta_attn_train_args* h_args, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Dropout whose decisions come from a counter (Philox4x32 with seven rounds) and are never stored (no counterpart in

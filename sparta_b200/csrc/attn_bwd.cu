@@ -1,0 +1,597 @@
+// Backward pass of the fused block-sparse attention (fp16 / bf16, head dim 64 or 128, 64 x 64 mask blocks).  The
+// probabilities are recomputed from Q, K and the forward pass's row log-sum-exp; nothing of size Nt x Ns is stored.
+//
+//   S = Q K^T    P = exp(scale S - lse)            on kept elements, 0 elsewhere
+//   P' = P keep up                                  (dropout: keep in {0, 1}, up = 1 / (1 - p))
+//   dV = P'^T dO     dP = (dO V^T) keep up     delta_i = sum_d dO_id O_id = sum_j P_ij dP_ij
+//   dS = P (dP - delta)      dQ = scale dS K       dK = scale dS^T Q        (K, V shared by heads: summed over them)
+//
+// Two passes over the kept blocks, each with its sums in tensor memory from the first block to the last, so that every
+// gradient is written once, in a fixed order of additions, without atomics and without a 32-bit workspace: one pass
+// owns 128 query rows and walks the kept key blocks (dQ), the other owns 128 key rows and walks the query blocks of
+// every head that shares them (dK, dV).  That is seven products per kept block instead of the five of a single pass,
+// which would have to add 128 x D 32-bit partial sums of dQ per block to global memory (in an order that changes from
+// run to run): 32 to 64 KB of atomic traffic per 128 x 128 scores, more than L2 takes at the rate of the products.
+//
+// Both passes are one kernel.  A CTA holds two resident tiles A1, A2 of 128 rows and streams pairs of 64-row blocks
+// B1, B2 through shared memory; the tile's rows are the lanes of tensor memory:
+//                      A1   A2   B1   B2
+//   dQ pass            Q    dO   K    V        S = A1 B1^T   dP = A2 B2^T   acc1 += dS B1
+//   dK, dV pass        K    V    Q    dO       S^T, dP^T likewise, acc1 = dK += dS^T B1, acc2 = dV += P'^T B2
+// P' and dS go back into tensor memory, over the columns that their own thread has just read, as the A operand of the
+// last products; B1 and B2 serve twice, K-major for S and dP, MN-major (the head dim contiguous) for the sums.
+//
+// Schedule.  A step is 64 columns of scores for 128 rows, one thread per row, in two phases: P from S, then dS from P
+// and dP.  One warp issues every MMA: when P of step j is in place, P'^T dO of j and then S of the next step; when dS
+// of j is in place, dS B1 of j and then dP of the next step.  MMAs of one thread execute in order, so S of the next
+// step may take the columns that P' is being read from, and the tensor pipe works on one half of a step while the
+// threads work on the other.  Head dim 64 takes 256 columns of tensor memory: two CTAs share an SM.  Head dim 128
+// fills tensor memory with one CTA, which has two groups of four warps and of score columns, taking turns.
+//   warps 0 .. 4 G - 1   scores and epilogue (G groups: group g takes steps g, g + G, ...)
+//   warp 4 G             TMA producer        warp 4 G + 1   MMA issue
+//
+// Masks and dropout are words of 32 decisions per row of the score matrix.  In the dK, dV pass a thread owns a key, so
+// each lane makes the word of one query row over the warp's 32 keys and the warp transposes the 32 x 32 bits.
+// The forward pass it belongs to: SparseAttention.forward (sparta/specializer/operators/sparse_attention.py:76-80),
+// whose gradients the reference takes through its three operators.
+#include <type_traits>
+
+#include "attn.cuh"
+#include "bsmm.cuh"
+#include "tc_common.cuh"
+
+namespace sparta {
+namespace {
+
+using namespace tc;
+
+constexpr int kBlk = 64;        // mask block edge = rows of B1, B2 per step
+constexpr int kTileM = 128;     // rows of A1, A2 per CTA (two blocks)
+constexpr int kMaxBlocks = 1024;  // blocks along the streamed side (65536 rows)
+
+struct BwdParams {
+  const int32_t* row_ptr;
+  const int32_t* idx;
+  const uint8_t* mask;      // [Nt, Ns] or null
+  const uint8_t* present;   // [Nt / 64, present_pitch]: block kept (built by the first kernel)
+  const float* neg_lse;     // [heads, Nt]: -lse * log2(e), -inf for a row without any score
+  const float* delta;       // [heads, Nt]
+  void* out1;               // dQ, or dK
+  void* out2;               // dV
+  int Nt, Ns, heads, kv_heads, group;
+  int present_pitch;
+  int by_head;              // launch order: tiles of a head together
+  float scale, scale_log2;
+  int32_t* status;
+  DropoutParams drop;
+};
+
+template <bool DKV, int D>
+struct BwdCfg {
+  static constexpr int kGroups = D == 64 ? 1 : 2;
+  static constexpr int kScoreWarps = 4 * kGroups;
+  static constexpr int kThreads = 32 * (kScoreWarps + 2);
+  static constexpr int kStages = 4;
+  static constexpr int kCtasPerSM = D == 64 ? 2 : 1;
+  static constexpr int kChunks = D / 64;               // 64-element (128-byte) chunks of the head dim
+  static constexpr int kABytes = kTileM * D * 2;
+  static constexpr int kBBytes = kBlk * D * 2;
+  static constexpr int kStatBytes = DKV ? 2 * kBlk * 4 : 0;  // neg_lse and delta of the streamed query rows
+  static constexpr int kStageBytes = 2 * kBBytes + kStatBytes;
+  static constexpr uint32_t kGroupCols = 2 * kBlk;     // S and dP of a group
+  static constexpr uint32_t kAcc1 = kGroups * kGroupCols, kAcc2 = kAcc1 + D;
+  static constexpr uint32_t kTmemCols = D == 64 ? 256 : 512;
+  static_assert(kAcc2 + (DKV ? D : 0) <= kTmemCols, "tensor memory budget");
+  static constexpr int kSmem = 2 * kABytes + kStages * 2 * kBBytes + kStages * kStatBytes + kMaxBlocks * 3 + 512 + 1024;
+};
+
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// delta and the negated log-sum-exp of every query row; the blocks kept, as bytes, for the pass that walks columns.
+// Bound by the read of O and dO.  A row is D / 8 lanes of 16 bytes.
+template <typename T, int D>
+__global__ void __launch_bounds__(256)
+attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const float* __restrict__ lse, float* __restrict__ neg_lse,
+                     float* __restrict__ delta, uint8_t* __restrict__ present, const int32_t* __restrict__ row_ptr,
+                     const int32_t* __restrict__ idx, long long rows, int nbr, int nbc, int pitch) {
+  constexpr int kLanes = D / 8;
+  const int lane = threadIdx.x % kLanes;
+  const long long row = (long long)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  float sum = 0.f;
+  if (row < rows) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(O + row * D) + lane);
+    const uint4 b = __ldg(reinterpret_cast<const uint4*>(dO + row * D) + lane);
+    const T* x = reinterpret_cast<const T*>(&a);
+    const T* y = reinterpret_cast<const T*>(&b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(to_float(x[i]), to_float(y[i]), sum);
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (row < rows && lane == 0) {
+    delta[row] = sum;
+    neg_lse[row] = lse[row] > -INFINITY ? lse[row] * -1.4426950408889634f : -INFINITY;
+  }
+  __shared__ uint8_t kept[kMaxBlocks];
+  for (int r = blockIdx.x; r < nbr; r += gridDim.x) {  // block rows of the mask
+    __syncthreads();
+    for (int c = threadIdx.x; c < pitch; c += 256) kept[c] = 0;
+    __syncthreads();
+    for (int e = row_ptr[r] + threadIdx.x; e < row_ptr[r + 1]; e += 256) {
+      const int c = __ldg(idx + e) & 0xffff;
+      if (c < nbc) kept[c] = 1;  // index arrays come from the caller: never index shared memory with them unchecked
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < pitch; c += 256) present[(long long)r * pitch + c] = kept[c];
+  }
+}
+
+template <bool DKV, int D, int FMT, bool MASK, bool DROP>
+__global__ void __launch_bounds__(BwdCfg<DKV, D>::kThreads, BwdCfg<DKV, D>::kCtasPerSM)
+attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant__ CUtensorMap tm_a2,
+                const __grid_constant__ CUtensorMap tm_b1, const __grid_constant__ CUtensorMap tm_b2, const BwdParams p) {
+  using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
+  using C = BwdCfg<DKV, D>;
+  constexpr int G = C::kGroups, kStages = C::kStages, kChunks = C::kChunks, kThreads = C::kThreads;
+  constexpr int kWarpLoad = C::kScoreWarps, kWarpMma = C::kScoreWarps + 1;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* a1_s = smem;
+  uint8_t* a2_s = a1_s + C::kABytes;
+  uint8_t* b1_s = a2_s + C::kABytes;                        // [kStages]
+  uint8_t* b2_s = b1_s + kStages * C::kBBytes;              // [kStages]
+  float* stat_s = reinterpret_cast<float*>(b2_s + kStages * C::kBBytes);  // [kStages][neg_lse 64, delta 64]
+  uint16_t* ulist = reinterpret_cast<uint16_t*>(b2_s + kStages * (C::kBBytes + C::kStatBytes));  // (block << 2) | presence bits
+  uint8_t* kmask = reinterpret_cast<uint8_t*>(ulist + kMaxBlocks);
+  uint64_t* a_full = reinterpret_cast<uint64_t*>(kmask + kMaxBlocks);
+  uint64_t* full = a_full + 1;          // [kStages] B1, B2 (and the statistics) of a step have landed
+  uint64_t* empty = full + kStages;     // [kStages] every MMA of the step is done
+  uint64_t* s_full = empty + kStages;   // [G] S complete
+  uint64_t* dp_full = s_full + G;       // [G] dP complete
+  uint64_t* p_full = dp_full + G;       // [G] S consumed (and P' in its place)
+  uint64_t* ds_full = p_full + G;       // [G] dS in place of dP
+  uint64_t* done = ds_full + G;         // the sums are complete
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
+  int* s_count = reinterpret_cast<int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows = DKV ? p.Ns : p.Nt;                  // of the resident side
+  const int heads = DKV ? p.kv_heads : p.heads;
+  const int tiles = (rows + kTileM - 1) / kTileM;
+  int head, tile;
+  if (!p.by_head) {  // the first tiles of all heads first: with global tokens they are the longest
+    tile = blockIdx.x / heads;
+    head = blockIdx.x - tile * heads;
+  } else {
+    head = blockIdx.x / tiles;
+    tile = blockIdx.x - head * tiles;
+  }
+  const int blk0 = tile * 2;                           // first of the tile's two blocks
+  const int nbr = p.Nt / kBlk, nbc = p.Ns / kBlk;
+  const int nstream = DKV ? nbr : nbc;
+
+  // ------------------------------ prologue ------------------------------
+  if (threadIdx.x == 0) {
+    mbar_init(a_full, 1);
+    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int g = 0; g < G; ++g) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&dp_full[g], 1);
+      mbar_init(&p_full[g], 4);
+      mbar_init(&ds_full[g], 4);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+  }
+  if (warp == kWarpLoad && lane == 0) {
+    prefetch_tensormap(&tm_a1);
+    prefetch_tensormap(&tm_a2);
+    prefetch_tensormap(&tm_b1);
+    prefetch_tensormap(&tm_b2);
+  }
+  if (warp == kWarpMma) tmem_alloc<C::kTmemCols>(tmem_holder);
+  if constexpr (DKV) {
+    for (int r = threadIdx.x; r < nbr; r += kThreads) {  // pitch is even: the two block columns are one 16-bit word
+      const uint32_t two = __ldg(reinterpret_cast<const uint16_t*>(p.present + (long long)r * p.present_pitch + blk0));
+      kmask[r] = static_cast<uint8_t>((two & 1u) | ((two >> 7) & 2u));
+    }
+  } else {
+    for (int k = threadIdx.x; k < nbc; k += kThreads) kmask[k] = 0;
+    __syncthreads();
+    // the two block rows are consecutive in the BCSR array: entry = (block row << 16) | key block
+    const int e1 = __ldg(p.row_ptr + min(blk0 + 2, nbr));
+    for (int e = __ldg(p.row_ptr + blk0) + threadIdx.x; e < e1; e += kThreads) {
+      const int v = __ldg(p.idx + e);
+      const int kb = v & 0xffff, r = static_cast<int>(static_cast<uint32_t>(v) >> 16) - blk0;
+      if (kb < nbc && r >= 0 && r < 2)
+        atomicOr(reinterpret_cast<unsigned int*>(kmask + (kb & ~3)), (1u << r) << (8 * (kb & 3)));
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {  // ordered compaction of the merged list
+    int n = 0;
+    for (int base = 0; base < nstream; base += 32) {
+      const int k = base + lane;
+      const int m = k < nstream ? kmask[k] : 0;
+      const unsigned bal = __ballot_sync(0xffffffffu, m != 0);
+      if (m) ulist[n + __popc(bal & ((1u << lane) - 1u))] = static_cast<uint16_t>((k << 2) | m);
+      n += __popc(bal);
+    }
+    if (lane == 0) *s_count = n;
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_holder;
+  const int count = *s_count;
+  const int steps = DKV ? count * p.group : count;     // dK, dV: the list once for every head that shares the keys
+  const long long a_row0 = (long long)head * rows + (long long)tile * kTileM;
+
+  bool failed = false;  // a bounded wait of this thread gave up
+  if (warp == kWarpLoad) {
+    // ------------------------------ producer ------------------------------
+    if (lane == 0 && steps > 0) {
+      mbar_arrive_expect_tx(a_full, 2 * C::kABytes);
+      for (int c = 0; c < kChunks; ++c) {
+        tma_load_2d(a1_s + c * (kTileM * 128), &tm_a1, c * 64, (int)a_row0, a_full);
+        tma_load_2d(a2_s + c * (kTileM * 128), &tm_a2, c * 64, (int)a_row0, a_full);
+      }
+      bool ok = true;
+      int h = 0, k = 0;  // step = h * count + k
+      for (int j = 0; j < steps; ++j) {
+        const int st = j % kStages;
+        if (!mbar_wait(&empty[st], ((j / kStages) & 1) ^ 1)) { ok = false; break; }
+        const long long row0 = DKV ? ((long long)head * p.group + h) * p.Nt : (long long)(head / p.group) * p.Ns;
+        const long long b_row = row0 + (ulist[k] >> 2) * kBlk;
+        mbar_arrive_expect_tx(&full[st], C::kStageBytes);
+        for (int c = 0; c < kChunks; ++c) {
+          tma_load_2d(b1_s + st * C::kBBytes + c * (kBlk * 128), &tm_b1, c * 64, (int)b_row, &full[st]);
+          tma_load_2d(b2_s + st * C::kBBytes + c * (kBlk * 128), &tm_b2, c * 64, (int)b_row, &full[st]);
+        }
+        if constexpr (DKV) {
+          bulk_load(stat_s + st * 2 * kBlk, p.neg_lse + b_row, kBlk * 4, &full[st]);
+          bulk_load(stat_s + st * 2 * kBlk + kBlk, p.delta + b_row, kBlk * 4, &full[st]);
+        }
+        if (++k == count) { k = 0; ++h; }
+      }
+      failed |= !ok;
+      if (!ok) atomicExch(&p.status[0], 1);
+    }
+  } else if (warp == kWarpMma) {
+    // ------------------------------ MMA issue ------------------------------
+    // K-major operands: 128-byte rows, 128-byte swizzle.  P', dS: A operands in tensor memory, lane = row, two 16-bit
+    // values per column, eight columns per K = 16 slab.  B1, B2 as right operands of the sums: MN-major (head dim
+    // contiguous), eight rows per 1024-byte group, 64-element chunks kBlk * 128 bytes apart.
+    const uint64_t desc_k = make_smem_desc(0, 16, 1024, SW_128B), desc_mn = make_smem_desc(0, kBlk * 128, 1024, SW_128B);
+    const uint32_t hi_k = static_cast<uint32_t>(desc_k >> 32), hi_mn = static_cast<uint32_t>(desc_mn >> 32);
+    const uint32_t flags_k = static_cast<uint32_t>(desc_k) & 0xffff0000u, flags_mn = static_cast<uint32_t>(desc_mn) & 0xffff0000u;
+    const uint32_t a1 = flags_k | (smem_u32(a1_s) >> 4), a2 = flags_k | (smem_u32(a2_s) >> 4);
+    const uint32_t b1 = smem_u32(b1_s) >> 4, b2 = smem_u32(b2_s) >> 4;
+    constexpr uint32_t idesc_s = make_idesc_f16(kTileM, kBlk, FMT, 0, 0), idesc_acc = make_idesc_f16(kTileM, D, FMT, 0, 1);
+    auto scores = [&](uint32_t d, uint32_t a, uint32_t b) {  // d = A B^T
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        umma_ss_lohi(d, a + (((kk / 4) * (kTileM * 128) + (kk % 4) * 32) >> 4), hi_k,
+                     flags_k | (b + (((kk / 4) * (kBlk * 128) + (kk % 4) * 32) >> 4)), hi_k, idesc_s, kk > 0 ? 1u : 0u);
+    };
+    auto accumulate = [&](uint32_t d, uint32_t a, uint32_t b, bool first) {  // d += A (tensor memory) B
+#pragma unroll
+      for (int kk = 0; kk < kBlk / 16; ++kk)
+        umma_ts_lohi(d, a + kk * 8, flags_mn | (b + ((kk * 16 * 128) >> 4)), hi_mn, idesc_acc, (!first || kk > 0) ? 1u : 0u);
+    };
+    bool ok = steps == 0 || mbar_wait(a_full, 0);
+    for (int j = 0; j < min(G, steps) && ok; ++j) {
+      if (!mbar_wait(&full[j], 0)) { ok = false; break; }
+      tc_fence_after_sync();
+      if (lane == 0) {
+        const uint32_t off = (j * C::kBBytes) >> 4, d = tmem_base + j * C::kGroupCols;
+        scores(d, a1, b1 + off);
+        umma_commit(&s_full[j]);
+        scores(d + kBlk, a2, b2 + off);
+        umma_commit(&dp_full[j]);
+      }
+      __syncwarp();
+    }
+    for (int j = 0; j < steps && ok; ++j) {
+      const int g = j % G, st = j % kStages, nx = (j + G) % kStages;
+      const uint32_t par = (j / G) & 1;
+      const uint32_t d = tmem_base + g * C::kGroupCols;
+      const uint32_t off = (st * C::kBBytes) >> 4, off_nx = (nx * C::kBBytes) >> 4;
+      const bool more = j + G < steps;
+      if (!mbar_wait(&p_full[g], par)) { ok = false; break; }
+      if (more && !mbar_wait(&full[nx], ((j + G) / kStages) & 1)) { ok = false; break; }
+      tc_fence_after_sync();
+      if (lane == 0) {
+        if constexpr (DKV) accumulate(tmem_base + C::kAcc2, d, b2 + off, j == 0);
+        if (more) {
+          scores(d, a1, b1 + off_nx);
+          umma_commit(&s_full[g]);
+        }
+      }
+      __syncwarp();
+      if (!mbar_wait(&ds_full[g], par)) { ok = false; break; }
+      tc_fence_after_sync();
+      if (lane == 0) {
+        accumulate(tmem_base + C::kAcc1, d + kBlk, b1 + off, j == 0);
+        umma_commit(&empty[st]);
+        if (more) {
+          scores(d + kBlk, a2, b2 + off_nx);
+          umma_commit(&dp_full[g]);
+        } else if (j + 1 == steps) {
+          umma_commit(done);
+        }
+      }
+      __syncwarp();
+    }
+    failed |= !ok;
+    if (!ok && lane == 0) atomicExch(&p.status[1], 1);
+  } else {
+    // ------------------------------ scores and epilogue ------------------------------
+    const int g = warp >> 2, quad = warp & 3;
+    const int row = quad * 32 + lane;                  // of the tile == tensor-memory lane
+    const int half = row >> 6;                         // which of the tile's two blocks (warp-uniform)
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t s_addr = tmem_base + lane_base + g * C::kGroupCols, dp_addr = s_addr + kBlk;
+    const int grow = tile * kTileM + row;              // row inside the head
+    const bool inside = grow < rows;
+    float neg_lse = 0.f, delta = 0.f;
+    if (!DKV && inside) {
+      neg_lse = __ldg(p.neg_lse + a_row0 + row);
+      delta = __ldg(p.delta + a_row0 + row);
+    }
+    PhiloxKey key = {};
+    uint32_t cut = 0;
+    const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
+    if constexpr (DROP) {
+      key = load_philox_key(p.drop);
+      cut = p.drop.threshold << 16;
+    }
+    const float up = p.drop.scale;
+    bool ok = true;
+    int h = 0, k = g;  // step = h * count + k
+    for (int j = g; j < steps; j += G, k += G) {
+      while (k >= count) { k -= count; ++h; }
+      const int st = j % kStages;
+      const uint32_t par = (j / G) & 1;
+      const int e = ulist[k];
+      const bool mine = (e >> half) & 1;               // the block is kept for this thread's rows (warp-uniform)
+      const int blk = e >> 2;
+      // words of decisions over this thread's 64 columns: made for a row of the score matrix (32 keys each), turned
+      // round where the thread is a key
+      uint32_t mask_w[2] = {0xffffffffu, 0xffffffffu}, keep_w[2] = {0xffffffffu, 0xffffffffu};
+      if ((MASK || DROP) && mine) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int q_row = DKV ? blk * kBlk + hh * 32 + lane : grow;
+          const int word = DKV ? tile * (kTileM / 32) + quad : blk * (kBlk / 32) + hh;
+          if constexpr (MASK) {
+            mask_w[hh] = mask_word32(p.mask + (long long)q_row * p.Ns + word * 32);
+            if constexpr (DKV) mask_w[hh] = transpose_bits32(mask_w[hh], lane);
+          }
+          if constexpr (DROP) {
+            const int q_head = DKV ? head * p.group + h : head;
+            keep_w[hh] = none ? 0u : philox_keep32(key, cut, word, q_row, q_head);
+            if constexpr (DKV) keep_w[hh] = transpose_bits32(keep_w[hh], lane);
+          }
+        }
+      }
+      if (ok && DKV && !mbar_wait_warp(&full[st], (j / kStages) & 1)) ok = false;  // the statistics are read here
+      if (ok && !mbar_wait_warp(&s_full[g], par)) ok = false;
+      if (!ok) continue;
+      tc_fence_after_sync();
+      // ---- P = exp2(scale log2(e) S - lse log2(e)) ----
+      const float4* nl4 = reinterpret_cast<const float4*>(stat_s + st * 2 * kBlk);
+      float prob[kBlk];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        uint32_t packed[16];
+        if (mine) {
+          uint32_t s[32];
+          tmem_ld_x32(s_addr + hh * 32, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float4 nl = make_float4(neg_lse, neg_lse, neg_lse, neg_lse);
+            if constexpr (DKV) nl = nl4[hh * 8 + i / 4];
+            const float n4[4] = {nl.x, nl.y, nl.z, nl.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float v = ex2_approx(fmaf(__uint_as_float(s[i + q]), p.scale_log2, n4[q]));
+              if constexpr (MASK) v = (mask_w[hh] >> (i + q)) & 1u ? v : 0.f;
+              prob[hh * 32 + i + q] = v;
+            }
+          }
+          if constexpr (DKV) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float v0 = prob[hh * 32 + 2 * i], v1 = prob[hh * 32 + 2 * i + 1];
+              if constexpr (DROP) {
+                v0 = (keep_w[hh] >> (2 * i)) & 1u ? v0 : 0.f;
+                v1 = (keep_w[hh] >> (2 * i + 1)) & 1u ? v1 : 0.f;
+              }
+              packed[i] = pack2<T>(v0, v1);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) packed[i] = 0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) prob[hh * 32 + i] = 0.f;
+        }
+        if constexpr (DKV) tmem_st_x16(s_addr + hh * 16, packed);  // over columns already read
+      }
+      if constexpr (DKV) tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[g]);
+      // ---- dS = P (dP - delta) ----
+      if (!mbar_wait_warp(&dp_full[g], par)) { ok = false; continue; }
+      tc_fence_after_sync();
+      const float4* dl4 = nl4 + kBlk / 4;
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        uint32_t packed[16];
+        if (mine) {
+          uint32_t s[32];
+          tmem_ld_x32(dp_addr + hh * 32, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float4 dl = make_float4(delta, delta, delta, delta);
+            if constexpr (DKV) dl = dl4[hh * 8 + i / 4];
+            const float d4[4] = {dl.x, dl.y, dl.z, dl.w};
+            float ds[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float v = __uint_as_float(s[i + q]);
+              if constexpr (DROP) v = (keep_w[hh] >> (i + q)) & 1u ? v * up : 0.f;
+              ds[q] = prob[hh * 32 + i + q] * (v - d4[q]);
+              // a masked score's probability is zero, and so is its dS whatever stands in V
+              if constexpr (MASK) ds[q] = (mask_w[hh] >> (i + q)) & 1u ? ds[q] : 0.f;
+            }
+            packed[i / 2] = pack2<T>(ds[0], ds[1]);
+            packed[i / 2 + 1] = pack2<T>(ds[2], ds[3]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) packed[i] = 0;
+        }
+        tmem_st_x16(dp_addr + hh * 16, packed);
+      }
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ds_full[g]);
+    }
+    // ---- epilogue: the sums -> global, one row per thread ----
+    if (ok && steps > 0 && !mbar_wait_warp(done, 0)) ok = false;
+    failed |= !ok;
+    if (!ok && lane == 0) atomicExch(&p.status[3], 1);
+    tc_fence_after_sync();
+    constexpr int kPieces = (DKV ? 2 : 1) * D / 32;    // 32-column pieces, dealt to the groups
+#pragma unroll
+    for (int c = 0; c < kPieces / G; ++c) {
+      const int piece = g * (kPieces / G) + c;
+      const bool second = piece >= D / 32;             // dV
+      const int col = (piece - (second ? D / 32 : 0)) * 32;
+      uint32_t r[32];
+      if (steps > 0 && ok) {
+        tmem_ld_x32(tmem_base + lane_base + C::kAcc1 + piece * 32, r);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = 0;
+      }
+      const float f = second ? (DROP ? up : 1.f) : p.scale;
+      uint32_t packed[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) packed[i] = pack2<T>(__uint_as_float(r[2 * i]) * f, __uint_as_float(r[2 * i + 1]) * f);
+      if (inside) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(second ? p.out2 : p.out1) + (a_row0 + row) * D + col);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          dst[q] = make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  sync_and_drain(failed);
+  if (warp == kWarpMma) {
+    tc_fence_after_sync();
+    tmem_dealloc<C::kTmemCols>(tmem_base);
+  }
+}
+
+int rows_map(CUtensorMap* map, const void* base, int dtype, int D, long long rows, uint32_t box_rows) {
+  const uint64_t dims[2] = {(uint64_t)D, (uint64_t)rows}, strides[1] = {(uint64_t)D * 2};
+  const uint32_t box[2] = {64, box_rows};
+  return make_tensor_map(map, base, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <bool DKV, int D, int FMT, bool MASK, bool DROP>
+int launch_pass(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2, const BwdParams& p,
+                cudaStream_t st) {
+  using C = BwdCfg<DKV, D>;
+  auto kern = attn_bwd_kernel<DKV, D, FMT, MASK, DROP>;
+  static SmemAttrOnce attr;
+  if (cudaError_t e = attr.ensure(kern, C::kSmem); e != cudaSuccess) return static_cast<int>(e);
+  const int rows = DKV ? p.Ns : p.Nt, heads = DKV ? p.kv_heads : p.heads;
+  const long long ctas = (long long)heads * ((rows + kTileM - 1) / kTileM);
+  kern<<<static_cast<unsigned>(ctas), C::kThreads, C::kSmem, st>>>(a1, a2, b1, b2, p);
+  return launch_status();
+}
+
+template <int D, int FMT, bool MASK, bool DROP>
+int launch_bwd(const AttnArgs& a, BwdParams p, float* neg_lse, float* delta, uint8_t* present, cudaStream_t st) {
+  using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
+  const long long q_rows = (long long)a.heads * a.Nt, k_rows = (long long)a.kv_heads * a.Ns;
+  const long long ctas = (q_rows + 2048 / D - 1) / (2048 / D);
+  attn_bwd_prep_kernel<T, D><<<static_cast<unsigned>(ctas), 256, 0, st>>>(
+      static_cast<const T*>(a.O), static_cast<const T*>(a.dO), a.lse, neg_lse, delta, present, a.row_ptr, a.idx, q_rows,
+      a.Nt / kBlk, a.Ns / kBlk, p.present_pitch);
+  if (int rc = launch_status(); rc != SPARTA_OK) return rc;
+  CUtensorMap q128, do128, k64, v64, k128, v128, q64, do64;
+  int rc = rows_map(&q128, a.Q, a.dtype, D, q_rows, kTileM);
+  if (rc == SPARTA_OK) rc = rows_map(&do128, a.dO, a.dtype, D, q_rows, kTileM);
+  if (rc == SPARTA_OK) rc = rows_map(&k64, a.K, a.dtype, D, k_rows, kBlk);
+  if (rc == SPARTA_OK) rc = rows_map(&v64, a.V, a.dtype, D, k_rows, kBlk);
+  if (rc == SPARTA_OK) rc = rows_map(&k128, a.K, a.dtype, D, k_rows, kTileM);
+  if (rc == SPARTA_OK) rc = rows_map(&v128, a.V, a.dtype, D, k_rows, kTileM);
+  if (rc == SPARTA_OK) rc = rows_map(&q64, a.Q, a.dtype, D, q_rows, kBlk);
+  if (rc == SPARTA_OK) rc = rows_map(&do64, a.dO, a.dtype, D, q_rows, kBlk);
+  if (rc != SPARTA_OK) return rc;
+  p.out1 = a.dK; p.out2 = a.dV;
+  p.by_head = kv_exceeds_l2(a.heads, a.Nt, D);
+  if (a.dK) rc = launch_pass<true, D, FMT, MASK, DROP>(k128, v128, q64, do64, p, st);
+  if (rc != SPARTA_OK || !a.dQ) return rc;
+  p.out1 = a.dQ; p.out2 = nullptr;
+  p.by_head = kv_exceeds_l2(a.kv_heads, a.Ns, D);
+  return launch_pass<false, D, FMT, MASK, DROP>(q128, do128, k64, v64, p, st);
+}
+
+template <int D, int FMT>
+int launch_variant(const AttnArgs& a, const BwdParams& p, float* neg_lse, float* delta, uint8_t* present, cudaStream_t st) {
+  const bool drop = p.drop.threshold > 0;
+  if (a.mask) return drop ? launch_bwd<D, FMT, true, true>(a, p, neg_lse, delta, present, st)
+                          : launch_bwd<D, FMT, true, false>(a, p, neg_lse, delta, present, st);
+  return drop ? launch_bwd<D, FMT, false, true>(a, p, neg_lse, delta, present, st)
+              : launch_bwd<D, FMT, false, false>(a, p, neg_lse, delta, present, st);
+}
+
+int present_pitch(int Ns) { return (Ns / kBlk + 1) & ~1; }
+size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
+size_t stat_bytes(int heads, int Nt) { return round16(sizeof(float) * (size_t)heads * Nt); }
+
+}  // namespace
+
+size_t attn_bwd_workspace(int heads, int Nt, int Ns) {
+  return 2 * stat_bytes(heads, Nt) + round16((size_t)(Nt / kBlk) * present_pitch(Ns));
+}
+
+int attn_bwd_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* status, cudaStream_t st) {
+  if (a.Ns / kBlk > kMaxBlocks || a.Nt / kBlk > kMaxBlocks) return SPARTA_ERR_UNSUPPORTED;
+  BwdParams p = {};
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  float* neg_lse = reinterpret_cast<float*>(ws);
+  float* delta = reinterpret_cast<float*>(ws + stat_bytes(a.heads, a.Nt));
+  uint8_t* present = ws + 2 * stat_bytes(a.heads, a.Nt);
+  p.row_ptr = a.row_ptr; p.idx = a.idx; p.mask = a.mask; p.present = present;
+  p.neg_lse = neg_lse; p.delta = delta;
+  p.Nt = a.Nt; p.Ns = a.Ns; p.heads = a.heads; p.kv_heads = a.kv_heads; p.group = a.heads / a.kv_heads;
+  p.present_pitch = present_pitch(a.Ns);
+  p.scale = a.scale; p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.status = status;
+  p.drop = drop;
+  if (a.D == 64)
+    return a.dtype == SPARTA_F16 ? launch_variant<64, 0>(a, p, neg_lse, delta, present, st)
+                                 : launch_variant<64, 1>(a, p, neg_lse, delta, present, st);
+  return a.dtype == SPARTA_F16 ? launch_variant<128, 0>(a, p, neg_lse, delta, present, st)
+                               : launch_variant<128, 1>(a, p, neg_lse, delta, present, st);
+}
+
+}  // namespace sparta

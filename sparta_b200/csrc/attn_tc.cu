@@ -22,6 +22,7 @@
 // producer, 9 issues the Q.K^T MMAs, 10 issues the P.V MMAs.  All mbarrier waits are bounded (status words of sparta_last_status).
 #include <type_traits>
 
+#include "attn.cuh"
 #include "bsmm.cuh"
 #include "tc_common.cuh"
 
@@ -39,15 +40,6 @@ constexpr int kThreads = 32 * (kSoftmaxWarps + 3);
 constexpr int kMaxKb = 1024;   // K blocks per row (Ns <= 65536)
 constexpr float kRescaleThreshold = 8.f;
 
-// 2^x by the special-function unit alone.  exp2f() wraps the same instruction in a range fix for
-// results below the normal range (a compare, two multiplies); probabilities that small round to zero
-// in fp16 / bf16 anyway, and the softmax warps are bound by the number of instructions they issue.
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 struct AttnParams {
   const int32_t* row_ptr;
   const int32_t* idx;
@@ -55,9 +47,11 @@ struct AttnParams {
   void* O;
   float* lse;
   int Nt, Ns, heads;
+  int group;            // query heads per key / value head
   int grouped;          // launch order, see the kernel
   float scale_log2;     // scale * log2(e)
   int32_t* status;
+  DropoutParams drop;   // on the probabilities, after the row sum
 };
 
 template <int D>
@@ -78,7 +72,7 @@ struct Cfg {
   static constexpr int kSmem = kQBytes + (kKStages + kVStages) * kKVBytes + kListBytes + 512 + 1024;
 };
 
-template <int D, int FMT>
+template <int D, int FMT, bool DROP>
 __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)  // D = 64: two CTAs per SM, 88 registers
 attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, AttnParams p) {
@@ -111,7 +105,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   __shared__ float s_lsum[2][kTileM];     // their partial row sums, at the end
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Launch order (see attn_tc2.cu): grouped by head when the K / V of all heads exceed L2, else head-major
-  const int tiles_per_head = p.Nt / kTileM;
+  const int tiles_per_head = (p.Nt + kTileM - 1) / kTileM;  // the last tile may be one block row high
   int head, tile;
   if (!p.grouped) {
     tile = blockIdx.x / p.heads;
@@ -136,7 +130,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     mbar_init(pv_done, 1);
     fence_mbar_init();
     s_range[0] = p.row_ptr[br0];
-    s_range[1] = p.row_ptr[br0 + 2];
+    s_range[1] = p.row_ptr[min(br0 + 2, p.Nt / kBlk)];
   }
   if (warp == kWarpLoad && lane == 0) {
     prefetch_tensormap(&tm_q);
@@ -172,7 +166,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const int count = *s_count;
   const int npairs = (count + 1) / 2;
   const long long q_row0 = (long long)head * p.Nt + (long long)tile * kTileM;
-  const long long kv_row0 = (long long)head * p.Ns;
+  const long long kv_row0 = (long long)(head / p.group) * p.Ns;
 
   bool failed = false;  // a bounded wait of this thread gave up
   if (warp == kWarpLoad) {
@@ -275,6 +269,13 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const long long grow = (long long)tile * kTileM + row;  // row inside the head
     constexpr int kOChunks = D / 64;           // 32-column chunks of O per thread
     float m_run = -INFINITY, l_run = 0.f;
+    PhiloxKey key = {};
+    uint32_t cut = 0;
+    const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
+    if constexpr (DROP) {
+      key = load_philox_key(p.drop);
+      cut = p.drop.threshold << 16;
+    }
     bool ok = true;
     for (int j = 0; j < npairs; ++j) {
       const int nblk = min(2, count - 2 * j);
@@ -370,29 +371,29 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         // every score of this row masked so far: subtracting +inf makes every probability zero
         const float neg_m = m_run > -INFINITY ? -m_run : -INFINITY;
         float sum = 0.f, sum1 = 0.f;
-        auto exp_pack = [&](const uint32_t* v, uint32_t* out) {  // 32 scores -> 16 packed pairs (out may be v)
+        auto exp_pack = [&](const uint32_t* v, uint32_t* out, int h) {  // scores 32 h .. -> 16 packed pairs (out may be v)
+          uint32_t keep = 0;
+          if constexpr (DROP) keep = none ? 0u : philox_keep32(key, cut, kb * (kBlk / 32) + h, (uint32_t)grow, head);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg_m));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg_m));
+            float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg_m));
+            float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg_m));
             // the row sum takes the fp32 probabilities: their rounding to 16 bits for P V is unbiased, and
             // converting them back cost two instructions per pair in warps bound by instruction issue
             // (two alternating partial sums keep the additions from forming one dependent chain)
             if (i & 1) sum1 += p0 + p1; else sum += p0 + p1;
-            if constexpr (FMT == 0) {
-              const __half2 hv = __floats2half2_rn(p0, p1);
-              out[i] = *reinterpret_cast<const uint32_t*>(&hv);
-            } else {
-              const __nv_bfloat162 hv = __floats2bfloat162_rn(p0, p1);
-              out[i] = *reinterpret_cast<const uint32_t*>(&hv);
+            if constexpr (DROP) {
+              p0 = (keep >> (2 * i)) & 1u ? p0 : 0.f;
+              p1 = (keep >> (2 * i + 1)) & 1u ? p1 : 0.f;
             }
+            out[i] = pack2<T>(p0, p1);
           }
         };
         const uint32_t p_addr = tmem_base + lane_base + C::kPCol + colhalf * (kBlk / 2);
         if constexpr (kHold) {
           if (mine) {
-            exp_pack(&r[0], &r[0]);
-            exp_pack(&r[32], &r[16]);
+            exp_pack(&r[0], &r[0], 0);
+            exp_pack(&r[32], &r[16], 1);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) r[i] = 0;
@@ -406,7 +407,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               tmem_ld_x32(s_addr + h * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
               tmem_ld_wait();
               if (p.mask) mask_scores(&r[0], h);
-              exp_pack(&r[0], packed);
+              exp_pack(&r[0], packed, h);
             } else {
 #pragma unroll
               for (int i = 0; i < 16; ++i) packed[i] = 0;
@@ -432,7 +433,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     s_lsum[colhalf][row] = l_run;  // the row sum is the two threads' partial sums
     named_barrier_sync(1, kSoftmaxWarps * 32);
     l_run += s_lsum[colhalf ^ 1][row];
-    const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+    const float inv = l_run > 0.f ? (DROP ? p.drop.scale : 1.f) / l_run : 0.f;
+    const bool inside = grow < p.Nt;
     T* orow = static_cast<T*>(p.O) + (q_row0 + row) * D;
 #pragma unroll
     for (int c = colhalf * kOChunks; c < (colhalf + 1) * kOChunks; ++c) {
@@ -448,20 +450,16 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float v0 = __uint_as_float(r[2 * i]) * inv, v1 = __uint_as_float(r[2 * i + 1]) * inv;
-        if constexpr (FMT == 0) {
-          const __half2 hv = __floats2half2_rn(v0, v1);
-          packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
-        } else {
-          const __nv_bfloat162 hv = __floats2bfloat162_rn(v0, v1);
-          packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
-        }
+        packed[i] = pack2<T>(v0, v1);
       }
-      uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+      if (inside) {
+        uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        dst[q] = make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+        for (int q = 0; q < 4; ++q)
+          dst[q] = make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+      }
     }
-    if (p.lse && colhalf == 0) {
+    if (p.lse && colhalf == 0 && inside) {
       // natural-log sum of exponentials of the scaled scores (-inf for a fully masked row)
       p.lse[(long long)head * p.Nt + grow] = l_run > 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
     }
@@ -474,31 +472,98 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   }
 }
 
-template <int D, int FMT>
-int launch_attn(const void* Q, const void* K, const void* V, const AttnParams& p, int dtype, cudaStream_t st) {
+template <int D, int FMT, bool DROP>
+int launch_attn(const AttnArgs& a, const AttnParams& p, cudaStream_t st) {
   using C = Cfg<D>;
   CUtensorMap tm_q, tm_k, tm_v;
   const uint64_t strides[1] = {(uint64_t)D * 2};
   {
-    const uint64_t dims[2] = {(uint64_t)D, (uint64_t)p.heads * p.Nt};
+    const uint64_t dims[2] = {(uint64_t)D, (uint64_t)a.heads * a.Nt};
     const uint32_t box[2] = {64, kTileM};
-    int rc = make_tensor_map(&tm_q, Q, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_tensor_map(&tm_q, a.Q, a.dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
   }
   {
-    const uint64_t dims[2] = {(uint64_t)D, (uint64_t)p.heads * p.Ns};
+    const uint64_t dims[2] = {(uint64_t)D, (uint64_t)a.kv_heads * a.Ns};
     const uint32_t box[2] = {64, kBlk};
-    int rc = make_tensor_map(&tm_k, K, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_tensor_map(&tm_k, a.K, a.dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
-    rc = make_tensor_map(&tm_v, V, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = make_tensor_map(&tm_v, a.V, a.dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
   }
-  auto kern = attn_fwd_tc_kernel<D, FMT>;
+  auto kern = attn_fwd_tc_kernel<D, FMT, DROP>;
   static SmemAttrOnce attr;
   if (cudaError_t e = attr.ensure(kern, C::kSmem); e != cudaSuccess) return static_cast<int>(e);
-  dim3 grid((unsigned)((long long)p.heads * (p.Nt / kTileM)));
+  dim3 grid((unsigned)((long long)p.heads * ((p.Nt + kTileM - 1) / kTileM)));
   kern<<<grid, kThreads, C::kSmem, st>>>(tm_q, tm_k, tm_v, p);
   return launch_status();
+}
+
+template <int D>
+int launch_one_tile(const AttnArgs& a, const DropoutParams& drop, int32_t* status, cudaStream_t st) {
+  AttnParams p;
+  p.row_ptr = a.row_ptr; p.idx = a.idx; p.mask = a.mask; p.O = a.O; p.lse = a.lse;
+  p.Nt = a.Nt; p.Ns = a.Ns; p.heads = a.heads;
+  p.group = a.heads / a.kv_heads;
+  p.grouped = kv_exceeds_l2(a.kv_heads, a.Ns, D);
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.status = status;
+  p.drop = drop;
+  if (drop.threshold > 0) return a.dtype == SPARTA_F16 ? launch_attn<D, 0, true>(a, p, st) : launch_attn<D, 1, true>(a, p, st);
+  return a.dtype == SPARTA_F16 ? launch_attn<D, 0, false>(a, p, st) : launch_attn<D, 1, false>(a, p, st);
+}
+
+int check_attn(const AttnArgs& a, int BLK) {
+  if (!a.Q || !a.K || !a.V || !a.O || !a.row_ptr || !a.idx || a.heads <= 0 || a.kv_heads <= 0 || a.Nt <= 0 || a.Ns <= 0)
+    return SPARTA_ERR_BAD_ARG;
+  if (a.dtype != SPARTA_F16 && a.dtype != SPARTA_BF16) return SPARTA_ERR_UNSUPPORTED;
+  if (BLK != kBlk || (a.D != 64 && a.D != 128)) return SPARTA_ERR_UNSUPPORTED;
+  if (a.Nt % kBlk || a.Ns % kBlk || a.heads % a.kv_heads) return SPARTA_ERR_SHAPE;
+  if (a.Ns / kBlk > kMaxKb || a.Nt / kTileM > 65535 || !(a.scale > 0.f)) return SPARTA_ERR_UNSUPPORTED;
+  if ((long long)a.heads * a.Nt > 0x7fffffffll || (long long)a.kv_heads * a.Ns > 0x7fffffffll) return SPARTA_ERR_SHAPE;
+  if (!aligned(a.Q, 16) || !aligned(a.K, 16) || !aligned(a.V, 16) || !aligned(a.O, 16)) return SPARTA_ERR_ALIGN;
+  if (a.mask && !aligned(a.mask, 16)) return SPARTA_ERR_ALIGN;
+  return SPARTA_OK;
+}
+
+int attn_fwd_entry(const AttnArgs& a, int BLK, const DropoutParams& drop, int32_t* status, void* const* copies, int n_copies,
+                   void* stream) {
+  if (int rc = check_attn(a, BLK); rc != SPARTA_OK) return rc;
+  if (!status) status = tc::device_status_ptr();
+  if (!status) return SPARTA_ERR_DRIVER;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // D = 128: two Q tiles per CTA sharing the K / V tiles (attn_tc2.cu), when the query length allows it.  D = 64
+  // stays with one tile per CTA and two CTAs per SM, which measured 25 % faster than the two-tile form there.
+  if (a.D == 128 && attn_tc2_supported(a.Nt)) return attn_tc2_launch(a, drop, status, copies, n_copies, st);
+  if (n_copies > 0) return SPARTA_ERR_UNSUPPORTED;  // the one-tile kernels store O only
+#ifdef SPARTA_ATTN64_TWO_BLOCKS
+  if (a.D == 64) return launch_one_tile<64>(a, drop, status, st);
+#endif
+  if (a.D == 64) return attn_tc64_launch(a, drop, status, st);
+  return launch_one_tile<128>(a, drop, status, st);
+}
+
+AttnArgs plain_args(const void* Q, const void* K, const void* V, void* O, const int32_t* row_ptr, const int32_t* bcsr_idx,
+                    const uint8_t* mask, float scale, int heads, int Nt, int Ns, int D, int dtype, float* lse) {
+  AttnArgs a = {};
+  a.Q = Q; a.K = K; a.V = V; a.O = O; a.lse = lse;
+  a.row_ptr = row_ptr; a.idx = bcsr_idx; a.mask = mask;
+  a.scale = scale;
+  a.heads = a.kv_heads = heads;
+  a.Nt = Nt; a.Ns = Ns; a.D = D; a.dtype = dtype;
+  return a;
+}
+
+int train_args(const sparta_attn_train_args* h, AttnArgs* a, DropoutParams* drop) {
+  if (!h) return SPARTA_ERR_BAD_ARG;
+  *a = plain_args(h->Q, h->K, h->V, h->O, h->row_ptr, h->bcsr_idx, h->mask, h->scale, h->heads, h->Nt, h->Ns, h->D, h->dtype,
+                  h->lse);
+  a->kv_heads = h->kv_heads;
+  a->dO = h->dO; a->dQ = h->dQ; a->dK = h->dK; a->dV = h->dV;
+  a->workspace = h->workspace;
+  if (!aligned(h->lse, 4) || (h->rng && !aligned(h->rng, 8))) return SPARTA_ERR_ALIGN;
+  if (!make_dropout(drop, h->dropout, h->rng, h->seed, h->call)) return SPARTA_ERR_BAD_ARG;
+  return check_attn(*a, h->BLK);
 }
 
 }  // namespace
@@ -511,19 +576,13 @@ using namespace sparta;
 
 extern "C" size_t sparta_attn_fwd_workspace_bytes(int, int, int, int, int) { return 0; }
 
-namespace {
-int attn_fwd_entry(const void* Q, const void* K, const void* V, void* O, const int32_t* row_ptr,
-                   const int32_t* bcsr_idx, const uint8_t* mask, float scale, int heads, int Nt, int Ns, int D,
-                   int BLK, int dtype, float* lse, int32_t* status, void* const* copies, int n_copies, void* stream);
-}
-
 extern "C" int sparta_attn_fwd(const void* Q, const void* K, const void* V, void* O, const int32_t* row_ptr,
                                const int32_t* bcsr_idx, const int32_t* nnz, const uint8_t* mask, float scale,
                                int heads, int Nt, int Ns, int D, int BLK, int dtype, float* lse,
                                int32_t* status, void* workspace, size_t workspace_bytes, void* stream) {
   (void)nnz; (void)workspace; (void)workspace_bytes;
-  return attn_fwd_entry(Q, K, V, O, row_ptr, bcsr_idx, mask, scale, heads, Nt, Ns, D, BLK, dtype, lse, status, nullptr, 0,
-                        stream);
+  return attn_fwd_entry(plain_args(Q, K, V, O, row_ptr, bcsr_idx, mask, scale, heads, Nt, Ns, D, dtype, lse), BLK, DropoutParams{},
+                        status, nullptr, 0, stream);
 }
 
 extern "C" int sparta_attn_fwd_gather(const void* Q, const void* K, const void* V, void* O, const int32_t* row_ptr,
@@ -532,42 +591,31 @@ extern "C" int sparta_attn_fwd_gather(const void* Q, const void* K, const void* 
                                       int32_t* status, void* const* copies, int n_copies, void* stream) {
   (void)nnz;
   if (n_copies < 0 || n_copies > SPARTA_ATTN_MAX_COPIES || (n_copies > 0 && !copies)) return SPARTA_ERR_BAD_ARG;
-  return attn_fwd_entry(Q, K, V, O, row_ptr, bcsr_idx, mask, scale, heads, Nt, Ns, D, BLK, dtype, lse, status, copies,
-                        n_copies, stream);
+  return attn_fwd_entry(plain_args(Q, K, V, O, row_ptr, bcsr_idx, mask, scale, heads, Nt, Ns, D, dtype, lse), BLK, DropoutParams{},
+                        status, copies, n_copies, stream);
 }
 
-namespace {
-int attn_fwd_entry(const void* Q, const void* K, const void* V, void* O, const int32_t* row_ptr,
-                   const int32_t* bcsr_idx, const uint8_t* mask, float scale, int heads, int Nt, int Ns, int D,
-                   int BLK, int dtype, float* lse, int32_t* status, void* const* copies, int n_copies, void* stream) {
-  if (!Q || !K || !V || !O || !row_ptr || !bcsr_idx || heads <= 0 || Nt <= 0 || Ns <= 0) return SPARTA_ERR_BAD_ARG;
-  if (dtype != SPARTA_F16 && dtype != SPARTA_BF16) return SPARTA_ERR_UNSUPPORTED;
-  if (BLK != kBlk || (D != 64 && D != 128)) return SPARTA_ERR_UNSUPPORTED;
-  if (Nt % kTileM || Ns % kBlk) return SPARTA_ERR_SHAPE;
-  if (Ns / kBlk > kMaxKb || Nt / kTileM > 65535 || !(scale > 0.f)) return SPARTA_ERR_UNSUPPORTED;
-  if ((long long)heads * Nt > 0x7fffffffll || (long long)heads * Ns > 0x7fffffffll) return SPARTA_ERR_SHAPE;
-  if (!aligned(Q, 16) || !aligned(K, 16) || !aligned(V, 16) || !aligned(O, 16)) return SPARTA_ERR_ALIGN;
-  if (mask && (!aligned(mask, 16) || Ns % 16)) return SPARTA_ERR_ALIGN;
-  AttnParams p;
-  p.row_ptr = row_ptr; p.idx = bcsr_idx; p.mask = mask; p.O = O; p.lse = lse;
-  p.Nt = Nt; p.Ns = Ns; p.heads = heads;
-  p.grouped = kv_exceeds_l2(heads, Ns, D);
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.status = status ? status : tc::device_status_ptr();
-  if (!p.status) return SPARTA_ERR_DRIVER;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // D = 128: two Q tiles per CTA sharing the K / V tiles (attn_tc2.cu), when the query length allows it.  D = 64
-  // stays with one tile per CTA and two CTAs per SM, which measured 25 % faster than the two-tile form there.
-  if (D == 128 && attn_tc2_supported(Nt))
-    return attn_tc2_launch(Q, K, V, O, row_ptr, bcsr_idx, mask, p.scale_log2, heads, Nt, Ns, D, dtype, lse, p.status,
-                           copies, n_copies, st);
-  if (n_copies > 0) return SPARTA_ERR_UNSUPPORTED;  // the one-tile kernels store O only
-#ifndef SPARTA_ATTN64_TWO_BLOCKS
-  if (D == 64)
-    return attn_tc64_launch(Q, K, V, O, row_ptr, bcsr_idx, mask, p.scale_log2, heads, Nt, Ns, dtype, lse, p.status, st);
-#endif
-  const int fmt = dtype == SPARTA_F16 ? 0 : 1;
-  if (D == 64) return fmt == 0 ? launch_attn<64, 0>(Q, K, V, p, dtype, st) : launch_attn<64, 1>(Q, K, V, p, dtype, st);
-  return fmt == 0 ? launch_attn<128, 0>(Q, K, V, p, dtype, st) : launch_attn<128, 1>(Q, K, V, p, dtype, st);
+extern "C" int sparta_attn_train_fwd(const sparta_attn_train_args* h_args, void* stream) {
+  AttnArgs a;
+  DropoutParams drop;
+  if (int rc = train_args(h_args, &a, &drop); rc != SPARTA_OK) return rc;
+  return attn_fwd_entry(a, h_args->BLK, drop, h_args->status, nullptr, 0, stream);
 }
-}  // namespace
+
+extern "C" size_t sparta_attn_train_bwd_workspace_bytes(int heads, int Nt, int Ns) {
+  if (heads <= 0 || Nt <= 0 || Ns <= 0) return 0;
+  return attn_bwd_workspace(heads, Nt, Ns);
+}
+
+extern "C" int sparta_attn_train_bwd(const sparta_attn_train_args* h_args, void* stream) {
+  AttnArgs a;
+  DropoutParams drop;
+  if (int rc = train_args(h_args, &a, &drop); rc != SPARTA_OK) return rc;
+  if (!a.lse || !a.dO || !a.dK != !a.dV || (!a.dQ && !a.dK)) return SPARTA_ERR_BAD_ARG;
+  if (!aligned(a.dO, 16) || !aligned(a.dQ, 16) || !aligned(a.dK, 16) || !aligned(a.dV, 16)) return SPARTA_ERR_ALIGN;
+  if (!a.workspace || h_args->workspace_bytes < attn_bwd_workspace(a.heads, a.Nt, a.Ns)) return SPARTA_ERR_WORKSPACE;
+  if (!aligned(a.workspace, 16)) return SPARTA_ERR_ALIGN;
+  int32_t* status = h_args->status ? h_args->status : tc::device_status_ptr();
+  if (!status) return SPARTA_ERR_DRIVER;
+  return attn_bwd_launch(a, drop, status, static_cast<cudaStream_t>(stream));
+}

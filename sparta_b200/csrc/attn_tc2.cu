@@ -28,6 +28,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "attn.cuh"
 #include "bsmm.cuh"
 #include "tc_common.cuh"
 
@@ -46,12 +47,6 @@ constexpr int kThreads = 32 * (kWarpLoad + 4);  // one idle warp rounds the CTA 
 constexpr int kMaxKb = 1024;   // K blocks per row (Ns <= 65536)
 constexpr float kRescaleThreshold = 8.f;
 constexpr int kStages = 2;
-
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 #ifdef SPARTA_ATTN_TRACE
 __device__ unsigned long long g_attn_trace[8][32];
@@ -75,9 +70,11 @@ struct Attn2Params {
   void* O;
   float* lse;
   int Nt, Ns, heads;
+  int group;            // query heads per key / value head
   int grouped;          // launch order, see the kernel
   float scale_log2;     // scale * log2(e)
   int32_t* status;
+  DropoutParams drop;   // on the probabilities, after the row sum
   int n_copies;         // further destinations of O (the peers' gathered outputs), see GatherMaps
 };
 
@@ -101,7 +98,7 @@ struct Cfg2 {
   static constexpr int kSmem = kTiles * kQBytes + 2 * kStages * kKVBytes + kListBytes + 512 + 1024;
 };
 
-template <int D, int FMT>
+template <int D, int FMT, bool DROP>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ GatherMaps gm, Attn2Params p) {
@@ -204,7 +201,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int count = *s_count;
   const int npairs = (count + 1) / 2;
   const long long q_row0 = (long long)head * p.Nt + (long long)cta_tile * (kTiles * kTileM);
-  const long long kv_row0 = (long long)head * p.Ns;
+  const long long kv_row0 = (long long)(head / p.group) * p.Ns;
 
   // presence bits of a step (both blocks of the pair): which tiles take part
   auto step_bits = [&](int j) -> uint32_t {
@@ -387,6 +384,13 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int bar_id = 1 + tile;
     constexpr int kOChunks = D / 64;           // 32-column chunks of O per thread
     float m_run = -INFINITY, l_run = 0.f;
+    PhiloxKey key = {};
+    uint32_t cut = 0;
+    const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
+    if constexpr (DROP) {
+      key = load_philox_key(p.drop);
+      cut = p.drop.threshold << 16;
+    }
     bool ok = true;
     int taken = 0;
     for (int j = 0; j < npairs; ++j) {
@@ -479,23 +483,23 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           for (int h = 0; h < 2; ++h) {
             uint32_t packed[16];
             if (mine) {
+              uint32_t keep = 0;
+              if constexpr (DROP) keep = none ? 0u : philox_keep32(key, cut, kb * (kBlk / 32) + h, (uint32_t)grow, head);
               tmem_ld_x32(s_addr + h * 32, r);
               tmem_ld_wait();
               if (p.mask) mask_scores(r, h);
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                const float p0 = ex2_approx(fmaf(__uint_as_float(r[2 * i]), p.scale_log2, neg_m));
-                const float p1 = ex2_approx(fmaf(__uint_as_float(r[2 * i + 1]), p.scale_log2, neg_m));
+                float p0 = ex2_approx(fmaf(__uint_as_float(r[2 * i]), p.scale_log2, neg_m));
+                float p1 = ex2_approx(fmaf(__uint_as_float(r[2 * i + 1]), p.scale_log2, neg_m));
                 // the row sum takes the fp32 probabilities (their rounding to 16 bits for P.V is unbiased); two
                 // alternating partial sums keep the additions from forming one dependent chain
                 if (i & 1) sum1 += p0 + p1; else sum += p0 + p1;
-                if constexpr (FMT == 0) {
-                  const __half2 hv = __floats2half2_rn(p0, p1);
-                  packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
-                } else {
-                  const __nv_bfloat162 hv = __floats2bfloat162_rn(p0, p1);
-                  packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
+                if constexpr (DROP) {
+                  p0 = (keep >> (2 * i)) & 1u ? p0 : 0.f;
+                  p1 = (keep >> (2 * i + 1)) & 1u ? p1 : 0.f;
                 }
+                packed[i] = pack2<T>(p0, p1);
               }
             } else {
 #pragma unroll
@@ -531,7 +535,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     s_lsum[tile][colhalf][row] = l_run;  // the row sum is the two threads' partial sums
     named_barrier_sync(bar_id, kSmWarps * 32);
     l_run += s_lsum[tile][colhalf ^ 1][row];
-    const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+    const float inv = l_run > 0.f ? (DROP ? p.drop.scale : 1.f) / l_run : 0.f;
     T* orow = static_cast<T*>(p.O) + (q_row0 + tile * kTileM + row) * D;
 #pragma unroll
     for (int c = colhalf * kOChunks; c < (colhalf + 1) * kOChunks; ++c) {
@@ -547,13 +551,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float v0 = __uint_as_float(o[2 * i]) * inv, v1 = __uint_as_float(o[2 * i + 1]) * inv;
-        if constexpr (FMT == 0) {
-          const __half2 hv = __floats2half2_rn(v0, v1);
-          packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
-        } else {
-          const __nv_bfloat162 hv = __floats2bfloat162_rn(v0, v1);
-          packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
-        }
+        packed[i] = pack2<T>(v0, v1);
       }
       uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
 #pragma unroll
@@ -593,9 +591,8 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   }
 }
 
-template <int D, int FMT>
-int launch_attn2(const void* Q, const void* K, const void* V, const Attn2Params& p, void* const* copies, int dtype,
-                 cudaStream_t st) {
+template <int D, int FMT, bool DROP>
+int launch_attn2(const AttnArgs& a, const Attn2Params& p, void* const* copies, cudaStream_t st) {
   using C = Cfg2<D>;
   CUtensorMap tm_q, tm_k, tm_v;
   GatherMaps gm;
@@ -604,25 +601,25 @@ int launch_attn2(const void* Q, const void* K, const void* V, const Attn2Params&
     const uint64_t dims[2] = {(uint64_t)D, (uint64_t)p.heads * p.Nt};
     const uint64_t pitch[1] = {(uint64_t)D * 2};
     const uint32_t box[2] = {64, kTileM};
-    int rc = make_tensor_map(&gm.m[g], copies[g], dtype, 2, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_tensor_map(&gm.m[g], copies[g], a.dtype, 2, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
   }
   const uint64_t strides[1] = {(uint64_t)D * 2};
   {
     const uint64_t dims[2] = {(uint64_t)D, (uint64_t)p.heads * p.Nt};
     const uint32_t box[2] = {64, kTileM};
-    int rc = make_tensor_map(&tm_q, Q, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_tensor_map(&tm_q, a.Q, a.dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
   }
   {
-    const uint64_t dims[2] = {(uint64_t)D, (uint64_t)p.heads * p.Ns};
+    const uint64_t dims[2] = {(uint64_t)D, (uint64_t)a.kv_heads * a.Ns};
     const uint32_t box[2] = {64, kBlk};
-    int rc = make_tensor_map(&tm_k, K, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_tensor_map(&tm_k, a.K, a.dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
-    rc = make_tensor_map(&tm_v, V, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = make_tensor_map(&tm_v, a.V, a.dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
   }
-  auto kern = attn_fwd_tc2_kernel<D, FMT>;
+  auto kern = attn_fwd_tc2_kernel<D, FMT, DROP>;
   static SmemAttrOnce attr;
   if (cudaError_t e = attr.ensure(kern, C::kSmem); e != cudaSuccess) return static_cast<int>(e);
   dim3 grid((unsigned)((long long)p.heads * (p.Nt / (kTiles * kTileM))));
@@ -639,22 +636,24 @@ bool kv_exceeds_l2(int heads, int Ns, int D) { return 4.0 * heads * Ns * D > 96.
 // The two-tile schedule applies when the query length is a multiple of 256 rows; attn_tc.cu takes the rest.
 bool attn_tc2_supported(int Nt) { return Nt % (kTiles * kTileM) == 0; }
 
-int attn_tc2_launch(const void* Q, const void* K, const void* V, void* O, const int32_t* row_ptr,
-                    const int32_t* bcsr_idx, const uint8_t* mask, float scale_log2, int heads, int Nt, int Ns,
-                    int D, int dtype, float* lse, int32_t* status, void* const* copies, int n_copies, cudaStream_t st) {
+int attn_tc2_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* status, void* const* copies, int n_copies,
+                    cudaStream_t st) {
   if (n_copies < 0 || n_copies > SPARTA_ATTN_MAX_COPIES || (n_copies > 0 && !copies)) return SPARTA_ERR_BAD_ARG;
   for (int g = 0; g < n_copies; ++g)
     if (!copies[g] || !aligned(copies[g], 16)) return SPARTA_ERR_ALIGN;
   Attn2Params p;
   p.n_copies = n_copies;
-  p.row_ptr = row_ptr; p.idx = bcsr_idx; p.mask = mask; p.O = O; p.lse = lse;
-  p.Nt = Nt; p.Ns = Ns; p.heads = heads;
-  p.grouped = kv_exceeds_l2(heads, Ns, D);
-  p.scale_log2 = scale_log2;
+  p.row_ptr = a.row_ptr; p.idx = a.idx; p.mask = a.mask; p.O = a.O; p.lse = a.lse;
+  p.Nt = a.Nt; p.Ns = a.Ns; p.heads = a.heads;
+  p.group = a.heads / a.kv_heads;
+  p.grouped = kv_exceeds_l2(a.kv_heads, a.Ns, a.D);
+  p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = status;
-  const int fmt = dtype == SPARTA_F16 ? 0 : 1;
-  if (D == 64) return fmt == 0 ? launch_attn2<64, 0>(Q, K, V, p, copies, dtype, st) : launch_attn2<64, 1>(Q, K, V, p, copies, dtype, st);
-  return fmt == 0 ? launch_attn2<128, 0>(Q, K, V, p, copies, dtype, st) : launch_attn2<128, 1>(Q, K, V, p, copies, dtype, st);
+  p.drop = drop;
+  if (a.D != 128) return SPARTA_ERR_UNSUPPORTED;
+  if (drop.threshold > 0)
+    return a.dtype == SPARTA_F16 ? launch_attn2<128, 0, true>(a, p, copies, st) : launch_attn2<128, 1, true>(a, p, copies, st);
+  return a.dtype == SPARTA_F16 ? launch_attn2<128, 0, false>(a, p, copies, st) : launch_attn2<128, 1, false>(a, p, copies, st);
 }
 
 }  // namespace sparta

@@ -16,6 +16,7 @@
 // Replaces the three launches of SparseAttention.forward (sparta/specializer/operators/sparse_attention.py:76-80).
 #include <type_traits>
 
+#include "attn.cuh"
 #include "bsmm.cuh"
 #include "tc_common.cuh"
 
@@ -48,18 +49,14 @@ struct Attn64Params {
   void* O;
   float* lse;
   int Nt, Ns, heads;
+  int group;            // query heads per key / value head
   int grouped;          // launch order: tiles of a head together when K / V of all heads exceed L2
   float scale_log2;     // scale * log2(e)
   int32_t* status;
+  DropoutParams drop;   // on the probabilities, after the row sum
 };
 
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-template <int FMT>
+template <int FMT, bool DROP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSM)
 attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, Attn64Params p) {
@@ -85,7 +82,7 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   int* s_range = s_count + 1;             // [2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles_per_head = p.Nt / kTileM;
+  const int tiles_per_head = (p.Nt + kTileM - 1) / kTileM;  // the last tile may be one block row high
   int head, tile;
   if (!p.grouped) {
     tile = blockIdx.x / p.heads;
@@ -112,7 +109,7 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     mbar_init(pv_done, 1);
     fence_mbar_init();
     s_range[0] = p.row_ptr[br0];
-    s_range[1] = p.row_ptr[br0 + 2];
+    s_range[1] = p.row_ptr[min(br0 + 2, p.Nt / kBlk)];
   }
   if (warp == kWarpLoad && lane == 0) {
     prefetch_tensormap(&tm_q);
@@ -147,7 +144,7 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const uint32_t tmem_base = *tmem_holder;
   const int count = *s_count;  // steps
   const long long q_row0 = (long long)head * p.Nt + (long long)tile * kTileM;
-  const long long kv_row0 = (long long)head * p.Ns;
+  const long long kv_row0 = (long long)(head / p.group) * p.Ns;
 
   bool failed = false;  // a bounded wait of this thread gave up
   if (warp == kWarpLoad) {
@@ -224,6 +221,13 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const uint32_t s_addr = tmem_base + lane_base;
     const long long grow = (long long)tile * kTileM + row;  // row inside the head
     float m_run = -INFINITY, l_run = 0.f;
+    PhiloxKey key = {};
+    uint32_t cut = 0;
+    const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
+    if constexpr (DROP) {
+      key = load_philox_key(p.drop);
+      cut = p.drop.threshold << 16;
+    }
     bool ok = true;
     for (int j = 0; j < count; ++j) {
       const int e = ulist[j];
@@ -295,6 +299,8 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       for (int h = 0; h < 2; ++h) {
         uint32_t packed[16];
         if (mine) {
+          uint32_t keep = 0;
+          if constexpr (DROP) keep = none ? 0u : philox_keep32(key, cut, kb * (kBlk / 32) + h, (uint32_t)grow, head);
           if constexpr (!kHold) {
             tmem_ld_x32(s_addr + h * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
             tmem_ld_wait();
@@ -303,16 +309,14 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           const uint32_t* v = kHold ? &r[32 * h] : &r[0];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg_m));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg_m));
+            float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg_m));
+            float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg_m));
             if (i & 1) sum1 += p0 + p1; else sum += p0 + p1;
-            if constexpr (FMT == 0) {
-              const __half2 hv = __floats2half2_rn(p0, p1);
-              packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
-            } else {
-              const __nv_bfloat162 hv = __floats2bfloat162_rn(p0, p1);
-              packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
+            if constexpr (DROP) {
+              p0 = (keep >> (2 * i)) & 1u ? p0 : 0.f;
+              p1 = (keep >> (2 * i + 1)) & 1u ? p1 : 0.f;
             }
+            packed[i] = pack2<T>(p0, p1);
           }
         } else {
 #pragma unroll
@@ -332,7 +336,8 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     failed |= !ok;
     if (!ok && lane == 0) atomicExch(&p.status[3], 1);
     tc_fence_after_sync();
-    const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+    const float inv = l_run > 0.f ? (DROP ? p.drop.scale : 1.f) / l_run : 0.f;
+    const bool inside = grow < p.Nt;
     T* orow = static_cast<T*>(p.O) + (q_row0 + row) * kD;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -348,20 +353,16 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float v0 = __uint_as_float(r[2 * i]) * inv, v1 = __uint_as_float(r[2 * i + 1]) * inv;
-        if constexpr (FMT == 0) {
-          const __half2 hv = __floats2half2_rn(v0, v1);
-          packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
-        } else {
-          const __nv_bfloat162 hv = __floats2bfloat162_rn(v0, v1);
-          packed[i] = *reinterpret_cast<const uint32_t*>(&hv);
-        }
+        packed[i] = pack2<T>(v0, v1);
       }
-      uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+      if (inside) {
+        uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        dst[q] = make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+        for (int q = 0; q < 4; ++q)
+          dst[q] = make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+      }
     }
-    if (p.lse) p.lse[(long long)head * p.Nt + grow] = l_run > 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
+    if (p.lse && inside) p.lse[(long long)head * p.Nt + grow] = l_run > 0.f ? (m_run + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
   }
   tc_fence_before_sync();
   sync_and_drain(failed);
@@ -371,44 +372,45 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   }
 }
 
-template <int FMT>
-int launch_attn64(const void* Q, const void* K, const void* V, const Attn64Params& p, int dtype, cudaStream_t st) {
+template <int FMT, bool DROP>
+int launch_attn64(const AttnArgs& a, const Attn64Params& p, cudaStream_t st) {
   CUtensorMap tm_q, tm_k, tm_v;
   const uint64_t strides[1] = {(uint64_t)kD * 2};
   {
-    const uint64_t dims[2] = {(uint64_t)kD, (uint64_t)p.heads * p.Nt};
+    const uint64_t dims[2] = {(uint64_t)kD, (uint64_t)a.heads * a.Nt};
     const uint32_t box[2] = {64, kTileM};
-    int rc = make_tensor_map(&tm_q, Q, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_tensor_map(&tm_q, a.Q, a.dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
   }
   {
-    const uint64_t dims[2] = {(uint64_t)kD, (uint64_t)p.heads * p.Ns};
+    const uint64_t dims[2] = {(uint64_t)kD, (uint64_t)a.kv_heads * a.Ns};
     const uint32_t box[2] = {64, kBlk};
-    int rc = make_tensor_map(&tm_k, K, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_tensor_map(&tm_k, a.K, a.dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
-    rc = make_tensor_map(&tm_v, V, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = make_tensor_map(&tm_v, a.V, a.dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != SPARTA_OK) return rc;
   }
-  auto kern = attn_fwd_tc64_kernel<FMT>;
+  auto kern = attn_fwd_tc64_kernel<FMT, DROP>;
   static SmemAttrOnce attr;
   if (cudaError_t e = attr.ensure(kern, kSmem); e != cudaSuccess) return static_cast<int>(e);
-  dim3 grid((unsigned)((long long)p.heads * (p.Nt / kTileM)));
+  dim3 grid((unsigned)((long long)p.heads * ((p.Nt + kTileM - 1) / kTileM)));
   kern<<<grid, kThreads, kSmem, st>>>(tm_q, tm_k, tm_v, p);
   return launch_status();
 }
 
 }  // namespace
 
-int attn_tc64_launch(const void* Q, const void* K, const void* V, void* O, const int32_t* row_ptr,
-                     const int32_t* bcsr_idx, const uint8_t* mask, float scale_log2, int heads, int Nt, int Ns,
-                     int dtype, float* lse, int32_t* status, cudaStream_t st) {
+int attn_tc64_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* status, cudaStream_t st) {
   Attn64Params p;
-  p.row_ptr = row_ptr; p.idx = bcsr_idx; p.mask = mask; p.O = O; p.lse = lse;
-  p.Nt = Nt; p.Ns = Ns; p.heads = heads;
-  p.grouped = kv_exceeds_l2(heads, Ns, kD);
-  p.scale_log2 = scale_log2;
+  p.row_ptr = a.row_ptr; p.idx = a.idx; p.mask = a.mask; p.O = a.O; p.lse = a.lse;
+  p.Nt = a.Nt; p.Ns = a.Ns; p.heads = a.heads;
+  p.group = a.heads / a.kv_heads;
+  p.grouped = kv_exceeds_l2(a.kv_heads, a.Ns, kD);
+  p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = status;
-  return dtype == SPARTA_F16 ? launch_attn64<0>(Q, K, V, p, dtype, st) : launch_attn64<1>(Q, K, V, p, dtype, st);
+  p.drop = drop;
+  if (drop.threshold > 0) return a.dtype == SPARTA_F16 ? launch_attn64<0, true>(a, p, st) : launch_attn64<1, true>(a, p, st);
+  return a.dtype == SPARTA_F16 ? launch_attn64<0, false>(a, p, st) : launch_attn64<1, false>(a, p, st);
 }
 
 }  // namespace sparta

@@ -4,13 +4,16 @@
 Two execution paths share the reference's API:
 
 * the composed path of the reference -- dds(Q, K^T) -> sparse softmax -> sdd(P, V), three kernels
-  that share one BCSR index set -- for every dtype and tile size, with backward;
-* the fused forward kernel (``sparta_attn_fwd``) for fp16 / bf16, E in {64, 128} and 64 x 64 tiles,
-  where the score tensor never reaches global memory.  It is chosen automatically when the
-  configuration allows it (``fused='auto'``) and provides no backward: with ``'auto'`` a forward whose
-  inputs require gradients takes the composed path.
+  that share one BCSR index set -- for every dtype and tile size;
+* the fused kernels (``sparta_attn_fwd``, and ``sparta_attn_train_fwd`` / ``sparta_attn_train_bwd`` for a
+  training step) for fp16 / bf16, E in {64, 128} and 64 x 64 tiles, where the score tensor never reaches
+  global memory: the forward pass keeps one number per row, the backward pass recomputes the probabilities.
+  They are chosen automatically when the configuration allows it (``fused='auto'``).
+
+Both take dropout on the probabilities (with the same decisions), key / value heads that several query heads
+share, and rotary positions, none of which the reference has.
 """
-from typing import Any, Dict, List, Optional
+from typing import Any, Dict, List, Optional, Tuple
 import os
 import warnings
 
@@ -21,22 +24,48 @@ from sparta_b200 import _lib
 from sparta_b200.specializer.operators.operator_base import OperatorBase
 from sparta_b200.specializer.operators.sparse_matmul import SparseBatchMatMul
 from sparta_b200.specializer.operators.sparse_softmax import SparseSoftmax
+from sparta_b200.specializer.operators.sparse_dropout import DropoutKey, SparseDropout, sparse_dropout
+from sparta_b200.specializer.operators.rotary import RotaryEmbedding
 from sparta_b200.specializer.kernels import KernelBase, PortConfig
 
 FUSED_BLOCK = 64
 FUSED_HEAD_DIMS = (64, 128)
+FUSED_DTYPES = (torch.float16, torch.bfloat16)
+
+
+#: 64 x 64 blocks along either side that the fused backward pass can list
+FUSED_MAX_BLOCKS = 1024
+
+
+def _rows(x: torch.Tensor, n: int) -> torch.Tensor:
+    """(..., n, E) as the contiguous, 16-byte aligned (heads, n, E) that the fused kernels read."""
+    x = x.reshape(-1, n, x.shape[-1]).contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 class _FusedAttentionFunc(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, op: 'SparseAttention', query, key, value):
-        return op._fused_forward(query.detach(), key.detach(), value.detach())
+    def forward(ctx, op: 'SparseAttention', query, key, value, p: float, rng: Optional[torch.Tensor], seed: int, call: int):
+        ctx.op, ctx.indexes, ctx.dropout = op, op._sparse_port.indexes, (p, seed, call)
+        ctx.shapes = query.shape, key.shape, value.shape
+        q, k, v = (_rows(x.detach(), n) for x, n in ((query, op._Nt), (key, op._Ns), (value, op._Ns)))
+        out, lse, mask = op._fused_train_forward(q, k, v, query.shape, p, DropoutKey(rng, seed, call))
+        # an element mask is read again: autograd refuses if it was rewritten in place since
+        ctx.save_for_backward(q, k, v, out, lse, mask, rng)
+        return out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        raise NotImplementedError(
-            'the fused sparse attention kernel has no backward; build with fused=False to train')
+        q, k, v, out, lse, mask, rng = ctx.saved_tensors
+        p, seed, call = ctx.dropout
+        want_q, want_kv = ctx.needs_input_grad[1], ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+        grads = ctx.op._fused_train_backward(q, k, v, out, lse, _rows(grad.detach(), q.shape[1]), ctx.indexes, mask, p,
+                                             DropoutKey(rng, seed, call), want_q, want_kv)
+        dq, dk, dv = (g if g is None else g.view(shape) for g, shape in zip(grads, ctx.shapes))
+        return (None, dq, dk if ctx.needs_input_grad[2] else None, dv if ctx.needs_input_grad[3] else None,
+                None, None, None, None)
 
 
 class SparseAttention(OperatorBase):
@@ -45,13 +74,23 @@ class SparseAttention(OperatorBase):
     Args:
         mask: :math:`(N_{target}, N_{source})` uint8 mask.
         fused: ``'auto'`` (default), ``True`` or ``False`` -- see the module docstring.
+        dropout: probability that a probability is dropped while the module is training (``SparseDropout``).
+        rotary: a ``RotaryEmbedding`` that turns queries and keys first.
 
-    Shape: Q :math:`(B \times H, N_{target}, E)`; K, V :math:`(B \times H, N_{source}, E)`;
-    output like Q.
+    ``forward(query, key, value, rng=None, positions=None, key_positions=None)``: ``rng`` replaces the module's own
+    random numbers (see ``SparseDropout``), the positions go to ``rotary``.  Inputs are finite: a NaN or an infinity
+    in a key or value row reaches every query row that shares a kept 64 x 64 block, or its neighbour in the same pair
+    of block rows, with it.
+
+    Shape: Q :math:`(B \times H, N_{target}, E)`; K, V :math:`(B \times H, N_{source}, E)`, or with fewer heads, each
+    shared by as many consecutive heads of Q; any leading dimensions; output like Q.
     """
 
-    def __init__(self, mask: torch.Tensor, fused: Any = 'auto'):
+    def __init__(self, mask: torch.Tensor, fused: Any = 'auto', dropout: float = 0.0,
+                 rotary: Optional[RotaryEmbedding] = None):
         super().__init__()
+        self._dropout = SparseDropout(dropout) if dropout else None
+        self.rotary = rotary
         self.mask = mask
         self._Nt, self._Ns = mask.shape
         self._matmul_qk = SparseBatchMatMul(C_mask=mask, transpose_A=False, transpose_B=True, compressed=True)
@@ -61,6 +100,7 @@ class SparseAttention(OperatorBase):
         self._fused_request = fused
         self._use_fused = False
         self._scale = 1.0
+        self._embed: Optional[int] = None
         self._attn_ws: Optional[torch.Tensor] = None
         self._attn_status: Optional[torch.Tensor] = None
         #: debugging aid: read the kernel's status words after every fused forward (one device
@@ -69,19 +109,101 @@ class SparseAttention(OperatorBase):
         self.ready = False
 
     # ---- forward paths ------------------------------------------------------------------
-    def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor):
+    def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, rng: Optional[torch.Tensor] = None,
+                positions: Optional[torch.Tensor] = None, key_positions: Optional[torch.Tensor] = None):
+        if self.rotary is not None:
+            query, key = self.rotary(query, key, positions=positions, key_positions=key_positions)
+        elif positions is not None or key_positions is not None:
+            raise ValueError('positions need a SparseAttention with rotary')
         if self.ready and self.dynamic:
             self._sparse_port.refresh()
-        if self.ready and self._use_fused:
-            # the fused kernel is forward-only: with fused='auto' a call that autograd will differentiate
-            # takes the three-operator path, which the reference trains through
-            # (test/unit/test_sparse_attention.py:86-92); fused=True keeps the fused kernel and raises in backward
+        p, numbers = 0.0, DropoutKey(None, 0, 0)
+        if self._dropout is not None and self.training and self._dropout.p > 0.0:
+            _lib.require_cuda(query)
+            p, numbers = self._dropout.p, self._dropout._counter.next(rng, query)
+        if self.ready and self._use_fused and (self._fused_request is True or query.dtype in FUSED_DTYPES):
+            group = self._check_heads(query, key, value)
             wants_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, value))
-            if self._fused_request is True or not wants_grad:
-                return _FusedAttentionFunc.apply(self, query, key, value)
+            if not wants_grad and p == 0.0 and group == 1:
+                return self._fused_forward(query.detach(), key.detach(), value.detach())
+            # the fused backward pass lists the blocks along both sides
+            if not wants_grad or self._fused_request is True or self._Nt // FUSED_BLOCK <= FUSED_MAX_BLOCKS:
+                return _FusedAttentionFunc.apply(self, query, key, value, p, *numbers)
+        shape = query.shape
+        if query.dim() != 3 or key.shape[:-2] != query.shape[:-2]:
+            query, key, value = self._flat_heads(query, key, value)
         qk = self._matmul_qk.forward(query, key)
         sm = self._softmax.forward(qk)
-        return self._matmul_out.forward(sm, value)
+        if p > 0.0:
+            sm = sparse_dropout(sm, p, numbers, self._sparse_port.indexes if self.ready else None)
+        out = self._matmul_out.forward(sm, value)
+        return out if out.shape == shape else out.reshape(shape)
+
+    def _check_heads(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> int:
+        """Query heads per key / value head; raises on shapes and types that do not belong together."""
+        q, k, v = (x.shape[:-2].numel() for x in (query, key, value))
+        if k != v or k == 0 or q % k:
+            raise ValueError(f'{q} query heads cannot share {k} key and {v} value heads')
+        E = query.shape[-1] if self._embed is None else self._embed
+        for x, n, name in ((query, self._Nt, 'query'), (key, self._Ns, 'key'), (value, self._Ns, 'value')):
+            if x.shape[-2] != n or x.shape[-1] != E:
+                raise ValueError(f'expect {name} shape (?, {n}, {E}), got {tuple(x.shape)}')
+            if x.dtype != query.dtype or x.device != query.device:
+                raise TypeError('query, key and value have to be of one type on one device')
+        return q // k
+
+    def _flat_heads(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> Tuple[torch.Tensor, ...]:
+        """(heads, N, E) for the composed path, shared key / value heads repeated."""
+        group = self._check_heads(query, key, value)
+        query, key, value = (x.reshape(-1, x.shape[-2], x.shape[-1]) for x in (query, key, value))
+        if group > 1:
+            key, value = key.repeat_interleave(group, 0), value.repeat_interleave(group, 0)
+        return query, key, value
+
+    def _train_args(self, q, k, v, out, lse, indexes, mask, p: float, numbers: DropoutKey) -> '_lib.AttnTrainArgs':
+        if self._attn_status is None or self._attn_status.device != q.device:
+            self._attn_status = torch.zeros(4, dtype=torch.int32, device=q.device)
+        return _lib.AttnTrainArgs(
+            Q=q.data_ptr(), K=k.data_ptr(), V=v.data_ptr(), O=out.data_ptr(), lse=lse.data_ptr(),
+            row_ptr=indexes.row_ptr.data_ptr(), bcsr_idx=indexes.bcsr_buf.data_ptr(), mask=_lib.ptr(mask),
+            rng=_lib.ptr(numbers.rng), seed=numbers.seed & 0xffffffffffffffff, call=numbers.call & 0xffffffff,
+            status=self._attn_status.data_ptr(), dropout=p, scale=self._scale, heads=q.shape[0], kv_heads=k.shape[0],
+            Nt=self._Nt, Ns=self._Ns, D=q.shape[2], BLK=FUSED_BLOCK, dtype=_lib.dtype_code(q))
+
+    def _raise_on_status(self):
+        if self.check_status and any(self.fused_status()):
+            raise RuntimeError(f'fused sparse attention: a bounded wait ran out on the device, status words '
+                               f'{self.fused_status()}; the output is invalid')
+
+    def _fused_train_forward(self, q, k, v, shape, p: float, numbers: DropoutKey):
+        _lib.require_cuda(q, k, v)
+        idx = self._sparse_port.indexes
+        mask = None if idx.block_uniform else idx.raw_mask
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        if out.numel() > 0:
+            with _lib.on_device(q.device):
+                _lib.check(_lib.lib().sparta_attn_train_fwd(self._train_args(q, k, v, out, lse, idx, mask, p, numbers),
+                                                            _lib.stream_ptr(q.device)), 'sparta_attn_train_fwd')
+            self._raise_on_status()
+        return out, lse, mask
+
+    def _fused_train_backward(self, q, k, v, out, lse, grad, indexes, mask, p: float, numbers: DropoutKey,
+                              want_q: bool, want_kv: bool):
+        dq = torch.empty_like(q) if want_q else None
+        dk, dv = (torch.empty_like(k), torch.empty_like(v)) if want_kv else (None, None)
+        if not (want_q or want_kv):
+            return dq, dk, dv
+        L = _lib.lib()
+        ws = torch.empty(L.sparta_attn_train_bwd_workspace_bytes(q.shape[0], self._Nt, self._Ns), dtype=torch.uint8,
+                         device=q.device)
+        args = self._train_args(q, k, v, out, lse, indexes, mask, p, numbers)
+        args.dO, args.dQ, args.dK, args.dV = grad.data_ptr(), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
+        with _lib.on_device(q.device):
+            _lib.check(L.sparta_attn_train_bwd(args, _lib.stream_ptr(q.device)), 'sparta_attn_train_bwd')
+        self._raise_on_status()
+        return dq, dk, dv
 
     def forward_gathered(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                          out: torch.Tensor, copies: List[int]) -> torch.Tensor:
@@ -157,14 +279,14 @@ class SparseAttention(OperatorBase):
 
     # ---- build ----------------------------------------------------------------------------
     def _fused_possible(self, config: Dict[str, Any], query: torch.Tensor) -> bool:
-        if query.dtype not in (torch.float16, torch.bfloat16) or query.shape[-1] not in FUSED_HEAD_DIMS:
+        if query.dtype not in FUSED_DTYPES or query.shape[-1] not in FUSED_HEAD_DIMS:
             return False
         qk, sm, out = config['qk/forward:C'], config['sm/forward:y'], config['out/forward:C']
         sizes = [qk.get('BLOCK_SIZE_M_VALUE'), qk.get('BLOCK_SIZE_N_VALUE'), sm.get('BLOCK_SIZE_H_VALUE'),
                  sm.get('BLOCK_SIZE_W_VALUE'), out.get('BLOCK_SIZE_M_VALUE'), out.get('BLOCK_SIZE_K_VALUE')]
         if any(s != FUSED_BLOCK for s in sizes):
             return False
-        if self._Nt % (2 * FUSED_BLOCK) or self._Ns % FUSED_BLOCK or self._Ns // FUSED_BLOCK > 1024:
+        if self._Nt % FUSED_BLOCK or self._Ns % FUSED_BLOCK or self._Ns // FUSED_BLOCK > FUSED_MAX_BLOCKS:
             return False
         return _lib.lib().sparta_tile_table(_lib.OP_ATTENTION, _lib.DTYPE_CODE[query.dtype], None, 0) > 0
 
@@ -172,7 +294,8 @@ class SparseAttention(OperatorBase):
         query, key, value = sample_inputs
         qB, kB, vB = (int(np.prod(t.shape[:-2])) for t in (query, key, value))
         (qN, qE), (kN, kE), (vN, vE) = (t.shape[-2:] for t in (query, key, value))
-        assert qB == kB == vB, 'query, key and value should have the same batch size'
+        assert kB == vB, 'key and value should have the same batch size'
+        assert kB > 0 and qB % kB == 0, 'the heads of query should be a multiple of those of key and value'
         assert self._Nt == qN, f'expect query shape (?, {self._Nt}, ?), got {query.shape}'
         assert self._Ns == kN, f'expect key shape (?, {self._Ns}, ?), got {key.shape}'
         assert self._Ns == vN, f'expect value shape (?, {self._Ns}, ?), got {value.shape}'
@@ -180,6 +303,7 @@ class SparseAttention(OperatorBase):
 
         self._softmax.set_temperature(np.sqrt(qE))
         self._scale = 1.0 / float(np.sqrt(qE))
+        self._embed = qE
 
         ops: Dict[str, OperatorBase] = {'qk': self._matmul_qk, 'sm': self._softmax, 'out': self._matmul_out}
         port_of = {'qk': 'C', 'sm': 'y', 'out': 'A'}
@@ -203,6 +327,9 @@ class SparseAttention(OperatorBase):
         # shapes of the intermediate tensors are not needed to bind prebuilt kernels, so no dense
         # pre-pass is run here (the reference computes qk and sm densely for shape inference)
         heads = qB
+        group = qB // kB
+        flat = lambda t, n: t.reshape(kB, n, qE).repeat_interleave(group, 0) if group > 1 else t.reshape(heads, n, qE)  # noqa: E731
+        key, value = flat(key.detach(), kN), flat(value.detach(), vN)
         qk_stub = torch.empty((heads, 0), dtype=query.dtype, device=query.device)
         sample = {'qk': [query.reshape(heads, qN, qE), key.reshape(heads, kN, kE)],
                   'sm': None, 'out': [qk_stub, value.reshape(heads, vN, vE)]}
@@ -226,6 +353,9 @@ class SparseAttention(OperatorBase):
     def set_sample_inputs(self, sample_inputs: List[torch.Tensor],
                           sample_grads: Optional[List[torch.Tensor]] = None):
         query, key, value = sample_inputs
+        if query.dim() != 3 or key.shape[:-2] != query.shape[:-2]:
+            query, key, value = (t.detach() for t in self._flat_heads(query, key, value))
+            sample_grads = None if sample_grads is None else [g.reshape(-1, *g.shape[-2:]) for g in sample_grads]
         self._softmax.set_temperature(np.sqrt(query.shape[-1]))
         if sample_grads is not None:
             query.requires_grad = True
