@@ -62,6 +62,39 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float v0, float v1) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// ---- words of 32 decisions about consecutive columns ----
+// In "split" order bit i is column 2 i and bit 16 + i column 2 i + 1: the two bits of a packed pair of 16-bit values are
+// 16 apart, so that one shift and one byte permutation make the mask of the pair.
+__device__ __forceinline__ uint32_t to_split32(uint32_t c) { return (c >> 1) | ((c & 1u) << 4); }        // column -> bit
+__device__ __forceinline__ uint32_t from_split32(uint32_t i) { return ((i & 15u) << 1) | (i >> 4); }  // bit -> column
+
+// 0xffff in each half whose bit (i, 16 + i) is set
+__device__ __forceinline__ uint32_t pair_mask(uint32_t word, int i) {
+  uint32_t m;
+  asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(m) : "r"(word << (15 - i)));  // sign of byte 1, byte 3 over two bytes each
+  return m;
+}
+
+// 32 dropout decisions of columns 32 g .. of a row, split order; threshold below 65536.  The 16-bit halves are compared
+// side by side: with the top bits set aside, a subtraction of the lower 15 bits leaves its borrow in place of the top
+// bit, and the result is decided by the top bits or, where they agree, by that.
+__device__ __forceinline__ uint32_t philox_split32(const PhiloxKey& key, uint32_t threshold, uint32_t g, uint32_t row, uint32_t batch) {
+  const uint32_t t = threshold * 0x00010001u, t15 = t & 0x7fff7fffu;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t w[4];
+    philox8(key, 4 * g + q, row, batch, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t d = (w[i] | 0x80008000u) - t15;
+      const uint32_t ge = (w[i] & ~t) | (~(w[i] ^ t) & d);
+      bits = (bits >> 1) | (ge & 0x80008000u);
+    }
+  }
+  return bits;
+}
+
 // 32 mask bytes (16-byte aligned) -> bit i set when byte i is not zero
 __device__ __forceinline__ uint32_t mask_word32(const uint8_t* m) {
   const uint4 lo = __ldg(reinterpret_cast<const uint4*>(m)), hi = __ldg(reinterpret_cast<const uint4*>(m) + 1);
@@ -74,6 +107,16 @@ __device__ __forceinline__ uint32_t mask_word32(const uint8_t* m) {
     bits |= (((t >> 7) * 0x10204080u) >> 28) << (4 * i);
   }
   return bits;
+}
+
+// the same in split order: the even bits gathered in the lower half, the odd ones in the upper
+__device__ __forceinline__ uint32_t mask_split32(const uint8_t* m) {
+  uint32_t x = mask_word32(m), t;
+  t = (x ^ (x >> 1)) & 0x22222222u; x ^= t ^ (t << 1);
+  t = (x ^ (x >> 2)) & 0x0c0c0c0cu; x ^= t ^ (t << 2);
+  t = (x ^ (x >> 4)) & 0x00f000f0u; x ^= t ^ (t << 4);
+  t = (x ^ (x >> 8)) & 0x0000ff00u; x ^= t ^ (t << 8);
+  return x;
 }
 
 // 32 x 32 bits across a warp, lane l holding row l: afterwards lane l holds column l (bit i = bit l of row i).  Swaps

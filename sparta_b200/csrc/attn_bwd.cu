@@ -21,17 +21,21 @@
 // P' and dS go back into tensor memory, over the columns that their own thread has just read, as the A operand of the
 // last products; B1 and B2 serve twice, K-major for S and dP, MN-major (the head dim contiguous) for the sums.
 //
-// Schedule.  A step is 64 columns of scores for 128 rows, one thread per row, in two phases: P from S, then dS from P
-// and dP.  One warp issues every MMA: when P of step j is in place, P'^T dO of j and then S of the next step; when dS
-// of j is in place, dS B1 of j and then dP of the next step.  MMAs of one thread execute in order, so S of the next
-// step may take the columns that P' is being read from, and the tensor pipe works on one half of a step while the
-// threads work on the other.  Head dim 64 takes 256 columns of tensor memory: two CTAs share an SM.  Head dim 128
-// fills tensor memory with one CTA, which has two groups of four warps and of score columns, taking turns.
-//   warps 0 .. 4 G - 1   scores and epilogue (G groups: group g takes steps g, g + G, ...)
-//   warp 4 G             TMA producer        warp 4 G + 1   MMA issue
+// Schedule.  A step is a pair of blocks, 128 columns of scores for 128 rows, in two phases: P from S, then dS from P and
+// dP; sixteen warps, four threads per row with 32 columns each.  One warp issues every MMA: when P of step j is in
+// place, P'^T dO of j and then S of a later step; when dS of j is in place, dS B1 of j and then dP of the next step.
+// MMAs of one thread execute in order, so S of a later step may take the columns that P' is being read from, and the
+// tensor pipe works on one half of a step while the threads work on the other.  Tensor memory: S 128 columns (twice for
+// head dim 64, so that the next S is never waited for), dP 128, the sums D each.
+//   Steps of one block (N = 64 instead of 128) make an MMA read 6 KB of shared memory for 32 cycles of math and double
+//   the number of MMAs, which one warp issues at one per 60 to 80 cycles: 1.6 times the time for head dim 128.
+//   The warp number and what MMAs are addressed with go through a shuffle: the compiler then knows them to be uniform
+//   and keeps descriptors in uniform registers (335 -> 305 us for dK, dV of B4 H16 S4096 D64 before the other steps).
+//   warps 0 .. 15  scores and epilogue        warp 16  TMA producer        warp 17  MMA issue
 //
-// Masks and dropout are words of 32 decisions per row of the score matrix.  In the dK, dV pass a thread owns a key, so
-// each lane makes the word of one query row over the warp's 32 keys and the warp transposes the 32 x 32 bits.
+// Masks and dropout are words of 32 decisions per row of the score matrix, even columns in the lower half.  In the
+// dK, dV pass a thread owns a key, so each lane makes the word of one query row over the warp's 32 keys and the warp
+// transposes the 32 x 32 bits.
 // The forward pass it belongs to: SparseAttention.forward (sparta/specializer/operators/sparse_attention.py:76-80),
 // whose gradients the reference takes through its three operators.
 #include <type_traits>
@@ -55,7 +59,7 @@ struct BwdParams {
   const uint8_t* mask;      // [Nt, Ns] or null
   const uint8_t* present;   // [Nt / 64, present_pitch]: block kept (built by the first kernel)
   const float* neg_lse;     // [heads, Nt]: -lse * log2(e), -inf for a row without any score
-  const float* delta;       // [heads, Nt]
+  const float* neg_delta;   // [heads, Nt]
   void* out1;               // dQ, or dK
   void* out2;               // dV
   int Nt, Ns, heads, kv_heads, group;
@@ -68,22 +72,47 @@ struct BwdParams {
 
 template <bool DKV, int D>
 struct BwdCfg {
-  static constexpr int kGroups = D == 64 ? 1 : 2;
-  static constexpr int kScoreWarps = 4 * kGroups;
-  static constexpr int kThreads = 32 * (kScoreWarps + 2);
-  static constexpr int kStages = 4;
+  static constexpr int kBlocks = D == 64 ? 1 : 2;      // blocks per step
+  static constexpr int kCols = kBlocks * kBlk;         // columns of a step
   static constexpr int kCtasPerSM = D == 64 ? 2 : 1;
+  static constexpr int kScoreWarps = 4 * (kCols / 32); // one per tensor-memory lane quadrant for each 32 columns of a step
+  static constexpr int kWarpLoad = kScoreWarps, kWarpMma = kScoreWarps + 1;
+  static constexpr int kThreads = 32 * (kScoreWarps + 2);
+  static constexpr int kSBuf = D == 64 && !DKV ? 2 : 1;      // score buffers in tensor memory
+  static constexpr int kStages = D == 64 ? 4 : 2;      // step j + kSBuf is read while j still is
   static constexpr int kChunks = D / 64;               // 64-element (128-byte) chunks of the head dim
   static constexpr int kABytes = kTileM * D * 2;
-  static constexpr int kBBytes = kBlk * D * 2;
-  static constexpr int kStatBytes = DKV ? 2 * kBlk * 4 : 0;  // neg_lse and delta of the streamed query rows
-  static constexpr int kStageBytes = 2 * kBBytes + kStatBytes;
-  static constexpr uint32_t kGroupCols = 2 * kBlk;     // S and dP of a group
-  static constexpr uint32_t kAcc1 = kGroups * kGroupCols, kAcc2 = kAcc1 + D;
-  static constexpr uint32_t kTmemCols = D == 64 ? 256 : 512;
+  static constexpr int kBBytes = kCols * D * 2;
+  static constexpr int kStatFloats = DKV ? 2 * kCols : 0;  // neg_lse and neg_delta of the streamed query rows
+  static constexpr uint32_t kDpCol = kSBuf * kCols;
+  static constexpr uint32_t kAcc1 = kDpCol + kCols, kAcc2 = kAcc1 + D;
+  static constexpr uint32_t kTmemCols = 512 / kCtasPerSM;
   static_assert(kAcc2 + (DKV ? D : 0) <= kTmemCols, "tensor memory budget");
-  static constexpr int kSmem = 2 * kABytes + kStages * 2 * kBBytes + kStages * kStatBytes + kMaxBlocks * 3 + 512 + 1024;
+  static constexpr int kSmem = 2 * kABytes + kStages * (2 * kBBytes + kStatFloats * 4) + kMaxBlocks * 3 + 512 + 1024;
 };
+
+// two 32-bit operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)), "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
 
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -91,12 +120,12 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                : "memory");
 }
 
-// delta and the negated log-sum-exp of every query row; the blocks kept, as bytes, for the pass that walks columns.
+// The negated delta and log-sum-exp of every query row; the blocks kept, as bytes, for the pass that walks columns.
 // Bound by the read of O and dO.  A row is D / 8 lanes of 16 bytes.
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const float* __restrict__ lse, float* __restrict__ neg_lse,
-                     float* __restrict__ delta, uint8_t* __restrict__ present, const int32_t* __restrict__ row_ptr,
+                     float* __restrict__ neg_delta, uint8_t* __restrict__ present, const int32_t* __restrict__ row_ptr,
                      const int32_t* __restrict__ idx, long long rows, int nbr, int nbc, int pitch) {
   constexpr int kLanes = D / 8;
   const int lane = threadIdx.x % kLanes;
@@ -113,7 +142,7 @@ attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const fl
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (row < rows && lane == 0) {
-    delta[row] = sum;
+    neg_delta[row] = -sum;
     neg_lse[row] = lse[row] > -INFINITY ? lse[row] * -1.4426950408889634f : -INFINITY;
   }
   __shared__ uint8_t kept[kMaxBlocks];
@@ -136,8 +165,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
                 const __grid_constant__ CUtensorMap tm_b1, const __grid_constant__ CUtensorMap tm_b2, const BwdParams p) {
   using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
   using C = BwdCfg<DKV, D>;
-  constexpr int G = C::kGroups, kStages = C::kStages, kChunks = C::kChunks, kThreads = C::kThreads;
-  constexpr int kWarpLoad = C::kScoreWarps, kWarpMma = C::kScoreWarps + 1;
+  constexpr int kSBuf = C::kSBuf, kStages = C::kStages, kChunks = C::kChunks, kThreads = C::kThreads;
+  constexpr int kScoreWarps = C::kScoreWarps, kWarpLoad = C::kWarpLoad, kWarpMma = C::kWarpMma;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -145,21 +174,24 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
   uint8_t* a2_s = a1_s + C::kABytes;
   uint8_t* b1_s = a2_s + C::kABytes;                        // [kStages]
   uint8_t* b2_s = b1_s + kStages * C::kBBytes;              // [kStages]
-  float* stat_s = reinterpret_cast<float*>(b2_s + kStages * C::kBBytes);  // [kStages][neg_lse 64, delta 64]
-  uint16_t* ulist = reinterpret_cast<uint16_t*>(b2_s + kStages * (C::kBBytes + C::kStatBytes));  // (block << 2) | presence bits
+  float* stat_s = reinterpret_cast<float*>(b2_s + kStages * C::kBBytes);  // [kStages][neg_lse 128, neg_delta 128]
+  uint16_t* ulist = reinterpret_cast<uint16_t*>(stat_s + kStages * C::kStatFloats);  // (block << 2) | presence bits
   uint8_t* kmask = reinterpret_cast<uint8_t*>(ulist + kMaxBlocks);
   uint64_t* a_full = reinterpret_cast<uint64_t*>(kmask + kMaxBlocks);
-  uint64_t* full = a_full + 1;          // [kStages] B1, B2 (and the statistics) of a step have landed
-  uint64_t* empty = full + kStages;     // [kStages] every MMA of the step is done
-  uint64_t* s_full = empty + kStages;   // [G] S complete
-  uint64_t* dp_full = s_full + G;       // [G] dP complete
-  uint64_t* p_full = dp_full + G;       // [G] S consumed (and P' in its place)
-  uint64_t* ds_full = p_full + G;       // [G] dS in place of dP
-  uint64_t* done = ds_full + G;         // the sums are complete
+  uint64_t* full1 = a_full + 1;         // [kStages] B1 (and the statistics) of a step have landed
+  uint64_t* empty1 = full1 + kStages;   // [kStages] the MMAs that read it are done
+  uint64_t* full2 = empty1 + kStages;   // [kStages] B2 likewise
+  uint64_t* empty2 = full2 + kStages;
+  uint64_t* s_full = empty2 + kStages;  // [kSBuf] S complete
+  uint64_t* dp_full = s_full + kSBuf;   // dP complete
+  uint64_t* p_full = dp_full + 1;       // [kSBuf] S consumed (and P' in its place); one for each buffer, since a warp
+                                        // may be done with the next S before another is with this one
+  uint64_t* ds_full = p_full + kSBuf;       // dS in place of dP
+  uint64_t* done = ds_full + 1;         // the sums are complete
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
   int* s_count = reinterpret_cast<int*>(tmem_holder + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rows = DKV ? p.Ns : p.Nt;                  // of the resident side
   const int heads = DKV ? p.kv_heads : p.heads;
   const int tiles = (rows + kTileM - 1) / kTileM;
@@ -178,13 +210,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
   // ------------------------------ prologue ------------------------------
   if (threadIdx.x == 0) {
     mbar_init(a_full, 1);
-    for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int g = 0; g < G; ++g) {
-      mbar_init(&s_full[g], 1);
-      mbar_init(&dp_full[g], 1);
-      mbar_init(&p_full[g], 4);
-      mbar_init(&ds_full[g], 4);
+    for (int st = 0; st < kStages; ++st) {
+      mbar_init(&full1[st], 1);
+      mbar_init(&empty1[st], 1);
+      mbar_init(&full2[st], 1);
+      mbar_init(&empty2[st], 1);
     }
+    for (int b = 0; b < kSBuf; ++b) { mbar_init(&s_full[b], 1); mbar_init(&p_full[b], kScoreWarps); }
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, kScoreWarps);
     mbar_init(done, 1);
     fence_mbar_init();
   }
@@ -227,9 +261,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_holder;
-  const int count = *s_count;
-  const int steps = DKV ? count * p.group : count;     // dK, dV: the list once for every head that shares the keys
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
+  const int count = __shfl_sync(0xffffffffu, *s_count, 0);
+  const int pairs = (count + C::kBlocks - 1) / C::kBlocks;  // steps through the list
+  const int steps = DKV ? pairs * p.group : pairs;     // dK, dV: the list once for every head that shares the keys
   const long long a_row0 = (long long)head * rows + (long long)tile * kTileM;
 
   bool failed = false;  // a bounded wait of this thread gave up
@@ -242,22 +277,30 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
         tma_load_2d(a2_s + c * (kTileM * 128), &tm_a2, c * 64, (int)a_row0, a_full);
       }
       bool ok = true;
-      int h = 0, k = 0;  // step = h * count + k
+      int h = 0, k = 0;  // step = h * pairs + k
       for (int j = 0; j < steps; ++j) {
-        const int st = j % kStages;
-        if (!mbar_wait(&empty[st], ((j / kStages) & 1) ^ 1)) { ok = false; break; }
+        const int st = j % kStages, nblk = min(C::kBlocks, count - C::kBlocks * k);
+        const uint32_t par = ((j / kStages) & 1) ^ 1;
         const long long row0 = DKV ? ((long long)head * p.group + h) * p.Nt : (long long)(head / p.group) * p.Ns;
-        const long long b_row = row0 + (ulist[k] >> 2) * kBlk;
-        mbar_arrive_expect_tx(&full[st], C::kStageBytes);
-        for (int c = 0; c < kChunks; ++c) {
-          tma_load_2d(b1_s + st * C::kBBytes + c * (kBlk * 128), &tm_b1, c * 64, (int)b_row, &full[st]);
-          tma_load_2d(b2_s + st * C::kBBytes + c * (kBlk * 128), &tm_b2, c * 64, (int)b_row, &full[st]);
+        if (!mbar_wait(&empty1[st], par)) { ok = false; break; }
+        mbar_arrive_expect_tx(&full1[st], nblk * (kBlk * D * 2 + (DKV ? 2 * kBlk * 4 : 0)));
+        for (int b = 0; b < nblk; ++b) {
+          const long long row = row0 + (ulist[C::kBlocks * k + b] >> 2) * kBlk;
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_2d(b1_s + st * C::kBBytes + c * (C::kCols * 128) + b * (kBlk * 128), &tm_b1, c * 64, (int)row, &full1[st]);
+          if constexpr (DKV) {
+            bulk_load(stat_s + st * C::kStatFloats + b * kBlk, p.neg_lse + row, kBlk * 4, &full1[st]);
+            bulk_load(stat_s + st * C::kStatFloats + C::kCols + b * kBlk, p.neg_delta + row, kBlk * 4, &full1[st]);
+          }
         }
-        if constexpr (DKV) {
-          bulk_load(stat_s + st * 2 * kBlk, p.neg_lse + b_row, kBlk * 4, &full[st]);
-          bulk_load(stat_s + st * 2 * kBlk + kBlk, p.delta + b_row, kBlk * 4, &full[st]);
+        if (!mbar_wait(&empty2[st], par)) { ok = false; break; }
+        mbar_arrive_expect_tx(&full2[st], nblk * kBlk * D * 2);
+        for (int b = 0; b < nblk; ++b) {
+          const long long row = row0 + (ulist[C::kBlocks * k + b] >> 2) * kBlk;
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_2d(b2_s + st * C::kBBytes + c * (C::kCols * 128) + b * (kBlk * 128), &tm_b2, c * 64, (int)row, &full2[st]);
         }
-        if (++k == count) { k = 0; ++h; }
+        if (++k == pairs) { k = 0; ++h; }
       }
       failed |= !ok;
       if (!ok) atomicExch(&p.status[0], 1);
@@ -265,218 +308,258 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
   } else if (warp == kWarpMma) {
     // ------------------------------ MMA issue ------------------------------
     // K-major operands: 128-byte rows, 128-byte swizzle.  P', dS: A operands in tensor memory, lane = row, two 16-bit
-    // values per column, eight columns per K = 16 slab.  B1, B2 as right operands of the sums: MN-major (head dim
-    // contiguous), eight rows per 1024-byte group, 64-element chunks kBlk * 128 bytes apart.
-    const uint64_t desc_k = make_smem_desc(0, 16, 1024, SW_128B), desc_mn = make_smem_desc(0, kBlk * 128, 1024, SW_128B);
+    // values per column, eight columns per K = 16 slab, the two slabs of each 32 columns at the first 16 of them.
+    // B1, B2 as right operands of the sums: MN-major (head dim contiguous), eight rows per 1024-byte group, 64-element
+    // chunks C::kCols * 128 bytes apart.
+    const uint64_t desc_k = make_smem_desc(0, 16, 1024, SW_128B), desc_mn = make_smem_desc(0, C::kCols * 128, 1024, SW_128B);
     const uint32_t hi_k = static_cast<uint32_t>(desc_k >> 32), hi_mn = static_cast<uint32_t>(desc_mn >> 32);
     const uint32_t flags_k = static_cast<uint32_t>(desc_k) & 0xffff0000u, flags_mn = static_cast<uint32_t>(desc_mn) & 0xffff0000u;
     const uint32_t a1 = flags_k | (smem_u32(a1_s) >> 4), a2 = flags_k | (smem_u32(a2_s) >> 4);
     const uint32_t b1 = smem_u32(b1_s) >> 4, b2 = smem_u32(b2_s) >> 4;
-    constexpr uint32_t idesc_s = make_idesc_f16(kTileM, kBlk, FMT, 0, 0), idesc_acc = make_idesc_f16(kTileM, D, FMT, 0, 1);
-    auto scores = [&](uint32_t d, uint32_t a, uint32_t b) {  // d = A B^T
+    constexpr uint32_t idesc_1 = make_idesc_f16(kTileM, kBlk, FMT, 0, 0), idesc_2 = make_idesc_f16(kTileM, 2 * kBlk, FMT, 0, 0);
+    constexpr uint32_t idesc_acc = make_idesc_f16(kTileM, D, FMT, 0, 1);
+    auto scores = [&](uint32_t d, uint32_t a, uint32_t b, int nblk) {  // d = A B^T
+      const uint32_t idesc = nblk == 2 ? idesc_2 : idesc_1;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        umma_ss_lohi(d, a + (((kk / 4) * (kTileM * 128) + (kk % 4) * 32) >> 4), hi_k,
-                     flags_k | (b + (((kk / 4) * (kBlk * 128) + (kk % 4) * 32) >> 4)), hi_k, idesc_s, kk > 0 ? 1u : 0u);
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off_a = ((kk / 4) * (kTileM * 128) + (kk % 4) * 32) >> 4;
+        const uint32_t off_b = ((kk / 4) * (C::kCols * 128) + (kk % 4) * 32) >> 4;
+        umma_ss_lohi(d, a + off_a, hi_k, flags_k | (b + off_b), hi_k, idesc, kk > 0 ? 1u : 0u);
+      }
     };
-    auto accumulate = [&](uint32_t d, uint32_t a, uint32_t b, bool first) {  // d += A (tensor memory) B
+    auto accumulate = [&](uint32_t d, uint32_t a, uint32_t b, int nblk, bool first) {  // d += A (tensor memory) B
 #pragma unroll
-      for (int kk = 0; kk < kBlk / 16; ++kk)
-        umma_ts_lohi(d, a + kk * 8, flags_mn | (b + ((kk * 16 * 128) >> 4)), hi_mn, idesc_acc, (!first || kk > 0) ? 1u : 0u);
+      for (int kk = 0; kk < C::kCols / 16; ++kk)
+        if (kk < nblk * (kBlk / 16))
+          umma_ts_lohi(d, a + (kk / 2) * 32 + (kk % 2) * 8, flags_mn | (b + ((kk * 16 * 128) >> 4)), hi_mn, idesc_acc,
+                       (!first || kk > 0) ? 1u : 0u);
     };
-    bool ok = steps == 0 || mbar_wait(a_full, 0);
-    for (int j = 0; j < min(G, steps) && ok; ++j) {
-      if (!mbar_wait(&full[j], 0)) { ok = false; break; }
+    // the last pair of the list may be a single block
+    auto blocks_of = [&](int j) { return C::kBlocks == 2 && !((count & 1) && (j + 1) % pairs == 0) ? 2 : 1; };
+    bool ok = steps == 0 || mbar_wait_warp(a_full, 0);
+#pragma unroll
+    for (int j = 0; j < kSBuf; ++j) {  // the first scores
+      if (j >= steps || !ok) break;
+      const int nblk = blocks_of(j);
+      if (!mbar_wait_warp(&full1[j], 0)) { ok = false; break; }
       tc_fence_after_sync();
-      if (lane == 0) {
-        const uint32_t off = (j * C::kBBytes) >> 4, d = tmem_base + j * C::kGroupCols;
-        scores(d, a1, b1 + off);
+      if (elect_one()) {
+        scores(tmem_base + j * C::kCols, a1, b1 + ((j * C::kBBytes) >> 4), nblk);
         umma_commit(&s_full[j]);
-        scores(d + kBlk, a2, b2 + off);
-        umma_commit(&dp_full[j]);
       }
       __syncwarp();
     }
-    for (int j = 0; j < steps && ok; ++j) {
-      const int g = j % G, st = j % kStages, nx = (j + G) % kStages;
-      const uint32_t par = (j / G) & 1;
-      const uint32_t d = tmem_base + g * C::kGroupCols;
-      const uint32_t off = (st * C::kBBytes) >> 4, off_nx = (nx * C::kBBytes) >> 4;
-      const bool more = j + G < steps;
-      if (!mbar_wait(&p_full[g], par)) { ok = false; break; }
-      if (more && !mbar_wait(&full[nx], ((j + G) / kStages) & 1)) { ok = false; break; }
-      tc_fence_after_sync();
-      if (lane == 0) {
-        if constexpr (DKV) accumulate(tmem_base + C::kAcc2, d, b2 + off, j == 0);
+    if (ok && steps > 0) {
+      ok = mbar_wait_warp(&full2[0], 0);
+      if (ok) {
+        tc_fence_after_sync();
+        if (elect_one()) {
+          scores(tmem_base + C::kDpCol, a2, b2, blocks_of(0));
+          umma_commit(dp_full);
+          if constexpr (!DKV) umma_commit(&empty2[0]);
+        }
+        __syncwarp();
+      }
+    }
+    // (unrolled over the stages, so that every descriptor is a compile-time offset from a base register)
+    for (int j0 = 0; j0 < steps && ok; j0 += kStages) {
+#pragma unroll
+      for (int st = 0; st < kStages; ++st) {
+        const int j = j0 + st, round = j0 / kStages;
+        if (j >= steps) break;
+        const uint32_t par = j & 1;
+        constexpr int kRing = kStages;
+        const int nx = (st + kSBuf) % kRing, nx2 = (st + 1) % kRing;
+        const uint32_t d = tmem_base + (j % kSBuf) * C::kCols, dp = tmem_base + C::kDpCol;
+        const uint32_t off = (st * C::kBBytes) >> 4;
+        const int nblk = blocks_of(j);
+        // ---- P of this step is in place: P' B2, then S of a later step ----
+        const bool more_s = j + kSBuf < steps;
+        if (!mbar_wait_warp(&p_full[j % kSBuf], (j / kSBuf) & 1)) { ok = false; break; }
+        tc_fence_after_sync();
+        if constexpr (DKV) {
+          if (elect_one()) {
+            accumulate(tmem_base + C::kAcc2, d, b2 + off, nblk, j == 0);
+            umma_commit(&empty2[st]);
+          }
+          __syncwarp();
+        }
+        if (more_s) {
+          if (!mbar_wait_warp(&full1[nx], (round + (st + kSBuf) / kRing) & 1)) { ok = false; break; }
+          tc_fence_after_sync();
+          if (elect_one()) {
+            scores(d, a1, b1 + ((nx * C::kBBytes) >> 4), blocks_of(j + kSBuf));
+            umma_commit(&s_full[j % kSBuf]);
+          }
+          __syncwarp();
+        }
+        // ---- dS of this step is in place: dS B1, then dP of the next step ----
+        const bool more = j + 1 < steps;
+        if (!mbar_wait_warp(ds_full, par)) { ok = false; break; }
+        tc_fence_after_sync();
+        if (elect_one()) {
+          accumulate(tmem_base + C::kAcc1, dp, b1 + off, nblk, j == 0);
+          umma_commit(&empty1[st]);
+          if (!more) umma_commit(done);
+        }
+        __syncwarp();
         if (more) {
-          scores(d, a1, b1 + off_nx);
-          umma_commit(&s_full[g]);
+          if (!mbar_wait_warp(&full2[nx2], (round + (st + 1) / kRing) & 1)) { ok = false; break; }
+          tc_fence_after_sync();
+          if (elect_one()) {
+            scores(dp, a2, b2 + ((nx2 * C::kBBytes) >> 4), blocks_of(j + 1));
+            umma_commit(dp_full);
+            if constexpr (!DKV) umma_commit(&empty2[nx2]);
+          }
+          __syncwarp();
         }
       }
-      __syncwarp();
-      if (!mbar_wait(&ds_full[g], par)) { ok = false; break; }
-      tc_fence_after_sync();
-      if (lane == 0) {
-        accumulate(tmem_base + C::kAcc1, d + kBlk, b1 + off, j == 0);
-        umma_commit(&empty[st]);
-        if (more) {
-          scores(d + kBlk, a2, b2 + off_nx);
-          umma_commit(&dp_full[g]);
-        } else if (j + 1 == steps) {
-          umma_commit(done);
-        }
-      }
-      __syncwarp();
     }
     failed |= !ok;
     if (!ok && lane == 0) atomicExch(&p.status[1], 1);
   } else {
     // ------------------------------ scores and epilogue ------------------------------
-    const int g = warp >> 2, quad = warp & 3;
+    const int quad = warp & 3, quarter = warp >> 2;    // lane quadrant, 32-column quarter of the step
     const int row = quad * 32 + lane;                  // of the tile == tensor-memory lane
-    const int half = row >> 6;                         // which of the tile's two blocks (warp-uniform)
+    const int half = quad >> 1;                        // which of the tile's two blocks
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_addr = tmem_base + lane_base + g * C::kGroupCols, dp_addr = s_addr + kBlk;
+    const uint32_t s_base = tmem_base + lane_base + quarter * 32, dp_addr = s_base + C::kDpCol;
     const int grow = tile * kTileM + row;              // row inside the head
     const bool inside = grow < rows;
-    float neg_lse = 0.f, delta = 0.f;
+    float2 nl = make_float2(0.f, 0.f), nd = nl;
     if (!DKV && inside) {
-      neg_lse = __ldg(p.neg_lse + a_row0 + row);
-      delta = __ldg(p.delta + a_row0 + row);
+      nl.x = nl.y = __ldg(p.neg_lse + a_row0 + row);
+      nd.x = nd.y = __ldg(p.neg_delta + a_row0 + row);
     }
     PhiloxKey key = {};
-    uint32_t cut = 0;
     const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
-    if constexpr (DROP) {
-      key = load_philox_key(p.drop);
-      cut = p.drop.threshold << 16;
-    }
+    if constexpr (DROP) key = load_philox_key(p.drop);
     const float up = p.drop.scale;
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
-    int h = 0, k = g;  // step = h * count + k
-    for (int j = g; j < steps; j += G, k += G) {
-      while (k >= count) { k -= count; ++h; }
-      const int st = j % kStages;
-      const uint32_t par = (j / G) & 1;
-      const int e = ulist[k];
-      const bool mine = (e >> half) & 1;               // the block is kept for this thread's rows (warp-uniform)
+    int h = 0, k = 0;  // step = h * pairs + k
+    for (int j = 0; j < steps; ++j) {
+      const int st = j % kStages, at = C::kBlocks * k + (quarter >> 1);
+      const int e = at < count ? ulist[at] : 0;
+      const bool there = at < count;                   // the pair has this block
+      const bool mine = (e >> half) & 1;               // it is kept for this warp's rows
       const int blk = e >> 2;
-      // words of decisions over this thread's 64 columns: made for a row of the score matrix (32 keys each), turned
-      // round where the thread is a key
-      uint32_t mask_w[2] = {0xffffffffu, 0xffffffffu}, keep_w[2] = {0xffffffffu, 0xffffffffu};
+      const uint32_t s_addr = s_base + (j % kSBuf) * C::kCols;
+      // words of decisions over this thread's 32 columns: made for a row of the score matrix, turned round where the
+      // thread is a key
+      uint32_t mask_w = 0xffffffffu, keep_w = 0xffffffffu;
       if ((MASK || DROP) && mine) {
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const int q_row = DKV ? blk * kBlk + hh * 32 + lane : grow;
-          const int word = DKV ? tile * (kTileM / 32) + quad : blk * (kBlk / 32) + hh;
-          if constexpr (MASK) {
-            mask_w[hh] = mask_word32(p.mask + (long long)q_row * p.Ns + word * 32);
-            if constexpr (DKV) mask_w[hh] = transpose_bits32(mask_w[hh], lane);
-          }
-          if constexpr (DROP) {
-            const int q_head = DKV ? head * p.group + h : head;
-            keep_w[hh] = none ? 0u : philox_keep32(key, cut, word, q_row, q_head);
-            if constexpr (DKV) keep_w[hh] = transpose_bits32(keep_w[hh], lane);
-          }
+        const int q_row = DKV ? blk * kBlk + (quarter & 1) * 32 + from_split32(lane) : grow;
+        const int word = DKV ? tile * (kTileM / 32) + quad : blk * (kBlk / 32) + (quarter & 1);
+        if constexpr (MASK) {
+          mask_w = mask_split32(p.mask + (long long)q_row * p.Ns + word * 32);
+          if constexpr (DKV) mask_w = __shfl_sync(0xffffffffu, transpose_bits32(mask_w, lane), to_split32(lane));
+        }
+        if constexpr (DROP) {
+          const int q_head = DKV ? head * p.group + h : head;
+          keep_w = none ? 0u : philox_split32(key, p.drop.threshold, word, q_row, q_head);
+          if constexpr (DKV) keep_w = __shfl_sync(0xffffffffu, transpose_bits32(keep_w, lane), to_split32(lane));
         }
       }
-      if (ok && DKV && !mbar_wait_warp(&full[st], (j / kStages) & 1)) ok = false;  // the statistics are read here
-      if (ok && !mbar_wait_warp(&s_full[g], par)) ok = false;
+      if (++k == pairs) { k = 0; ++h; }
+      if (ok && DKV && !mbar_wait_warp(&full1[st], (j / kStages) & 1)) ok = false;  // the statistics are read here
+      if (ok && !mbar_wait_warp(&s_full[j % kSBuf], (j / kSBuf) & 1)) ok = false;
       if (!ok) continue;
       tc_fence_after_sync();
       // ---- P = exp2(scale log2(e) S - lse log2(e)) ----
-      const float4* nl4 = reinterpret_cast<const float4*>(stat_s + st * 2 * kBlk);
-      float prob[kBlk];
+      const float4* nl4 = reinterpret_cast<const float4*>(stat_s + st * C::kStatFloats + quarter * 32);
+      float2 prob[16];
+      uint32_t packed[16];
+      if (mine) {
+        uint32_t s[32];
+        tmem_ld_x32(s_addr, s);
+        tmem_ld_wait();
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        uint32_t packed[16];
-        if (mine) {
-          uint32_t s[32];
-          tmem_ld_x32(s_addr + hh * 32, s);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float4 nl = make_float4(neg_lse, neg_lse, neg_lse, neg_lse);
-            if constexpr (DKV) nl = nl4[hh * 8 + i / 4];
-            const float n4[4] = {nl.x, nl.y, nl.z, nl.w};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float v = ex2_approx(fmaf(__uint_as_float(s[i + q]), p.scale_log2, n4[q]));
-              if constexpr (MASK) v = (mask_w[hh] >> (i + q)) & 1u ? v : 0.f;
-              prob[hh * 32 + i + q] = v;
-            }
-          }
+        for (int i = 0; i < 16; i += 2) {
+          float2 n0 = nl, n1 = nl;
           if constexpr (DKV) {
+            const float4 n = nl4[i / 2];
+            n0 = make_float2(n.x, n.y);
+            n1 = make_float2(n.z, n.w);
+          }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float v0 = prob[hh * 32 + 2 * i], v1 = prob[hh * 32 + 2 * i + 1];
-              if constexpr (DROP) {
-                v0 = (keep_w[hh] >> (2 * i)) & 1u ? v0 : 0.f;
-                v1 = (keep_w[hh] >> (2 * i + 1)) & 1u ? v1 : 0.f;
-              }
-              packed[i] = pack2<T>(v0, v1);
+          for (int q = 0; q < 2; ++q) {
+            float2 v = fma2(make_float2(__uint_as_float(s[2 * (i + q)]), __uint_as_float(s[2 * (i + q) + 1])), scale2, q ? n1 : n0);
+            v.x = ex2_approx(v.x);
+            v.y = ex2_approx(v.y);
+            if constexpr (MASK) {
+              v.x = (mask_w >> (i + q)) & 1u ? v.x : 0.f;
+              v.y = (mask_w >> (i + q + 16)) & 1u ? v.y : 0.f;
+            }
+            prob[i + q] = v;
+            if constexpr (DKV) {
+              packed[i + q] = pack2<T>(v.x, v.y);
+              if constexpr (DROP) packed[i + q] &= pair_mask(keep_w, i + q);
             }
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) packed[i] = 0;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) prob[hh * 32 + i] = 0.f;
         }
-        if constexpr (DKV) tmem_st_x16(s_addr + hh * 16, packed);  // over columns already read
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) packed[i] = 0;
       }
-      if constexpr (DKV) tmem_st_wait();
+      if constexpr (DKV) {
+        if (there) {
+          tmem_st_x16(s_addr, packed);  // over columns that this thread has read
+          tmem_st_wait();
+        }
+      }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[g]);
+      if (lane == 0) mbar_arrive(&p_full[j % kSBuf]);
       // ---- dS = P (dP - delta) ----
-      if (!mbar_wait_warp(&dp_full[g], par)) { ok = false; continue; }
+      if (!mbar_wait_warp(dp_full, j & 1)) { ok = false; continue; }
       tc_fence_after_sync();
-      const float4* dl4 = nl4 + kBlk / 4;
+      const float4* nd4 = nl4 + C::kCols / 4;
+      if (mine) {
+        uint32_t s[32];
+        tmem_ld_x32(dp_addr, s);
+        tmem_ld_wait();
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        uint32_t packed[16];
-        if (mine) {
-          uint32_t s[32];
-          tmem_ld_x32(dp_addr + hh * 32, s);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float4 dl = make_float4(delta, delta, delta, delta);
-            if constexpr (DKV) dl = dl4[hh * 8 + i / 4];
-            const float d4[4] = {dl.x, dl.y, dl.z, dl.w};
-            float ds[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float v = __uint_as_float(s[i + q]);
-              if constexpr (DROP) v = (keep_w[hh] >> (i + q)) & 1u ? v * up : 0.f;
-              ds[q] = prob[hh * 32 + i + q] * (v - d4[q]);
-              // a masked score's probability is zero, and so is its dS whatever stands in V
-              if constexpr (MASK) ds[q] = (mask_w[hh] >> (i + q)) & 1u ? ds[q] : 0.f;
-            }
-            packed[i / 2] = pack2<T>(ds[0], ds[1]);
-            packed[i / 2 + 1] = pack2<T>(ds[2], ds[3]);
+        for (int i = 0; i < 16; i += 2) {
+          float2 n0 = nd, n1 = nd;
+          if constexpr (DKV) {
+            const float4 n = nd4[i / 2];
+            n0 = make_float2(n.x, n.y);
+            n1 = make_float2(n.z, n.w);
           }
-        } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) packed[i] = 0;
+          for (int q = 0; q < 2; ++q) {
+            float2 v = make_float2(__uint_as_float(s[2 * (i + q)]), __uint_as_float(s[2 * (i + q) + 1]));
+            if constexpr (DROP) {
+              v = mul2(v, make_float2(up, up));
+              v.x = (keep_w >> (i + q)) & 1u ? v.x : 0.f;
+              v.y = (keep_w >> (i + q + 16)) & 1u ? v.y : 0.f;
+            }
+            v = mul2(prob[i + q], add2(v, q ? n1 : n0));
+            packed[i + q] = pack2<T>(v.x, v.y);
+            // a masked score's probability is zero, and so is its dS whatever stands in V
+            if constexpr (MASK) packed[i + q] &= pair_mask(mask_w, i + q);
+          }
         }
-        tmem_st_x16(dp_addr + hh * 16, packed);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) packed[i] = 0;
       }
-      tmem_st_wait();
+      if (there) {
+        tmem_st_x16(dp_addr, packed);
+        tmem_st_wait();
+      }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ds_full[g]);
+      if (lane == 0) mbar_arrive(ds_full);
     }
     // ---- epilogue: the sums -> global, one row per thread ----
     if (ok && steps > 0 && !mbar_wait_warp(done, 0)) ok = false;
     failed |= !ok;
     if (!ok && lane == 0) atomicExch(&p.status[3], 1);
     tc_fence_after_sync();
-    constexpr int kPieces = (DKV ? 2 : 1) * D / 32;    // 32-column pieces, dealt to the groups
-#pragma unroll
-    for (int c = 0; c < kPieces / G; ++c) {
-      const int piece = g * (kPieces / G) + c;
+    constexpr int kPieces = (DKV ? 2 : 1) * D / 32;    // 32-column pieces, dealt to the four threads of a row
+    for (int piece = quarter; piece < kPieces; piece += kScoreWarps / 4) {
       const bool second = piece >= D / 32;             // dV
       const int col = (piece - (second ? D / 32 : 0)) * 32;
       uint32_t r[32];
@@ -527,12 +610,12 @@ int launch_pass(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap&
 }
 
 template <int D, int FMT, bool MASK, bool DROP>
-int launch_bwd(const AttnArgs& a, BwdParams p, float* neg_lse, float* delta, uint8_t* present, cudaStream_t st) {
+int launch_bwd(const AttnArgs& a, BwdParams p, float* neg_lse, float* neg_delta, uint8_t* present, cudaStream_t st) {
   using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
   const long long q_rows = (long long)a.heads * a.Nt, k_rows = (long long)a.kv_heads * a.Ns;
   const long long ctas = (q_rows + 2048 / D - 1) / (2048 / D);
   attn_bwd_prep_kernel<T, D><<<static_cast<unsigned>(ctas), 256, 0, st>>>(
-      static_cast<const T*>(a.O), static_cast<const T*>(a.dO), a.lse, neg_lse, delta, present, a.row_ptr, a.idx, q_rows,
+      static_cast<const T*>(a.O), static_cast<const T*>(a.dO), a.lse, neg_lse, neg_delta, present, a.row_ptr, a.idx, q_rows,
       a.Nt / kBlk, a.Ns / kBlk, p.present_pitch);
   if (int rc = launch_status(); rc != SPARTA_OK) return rc;
   CUtensorMap q128, do128, k64, v64, k128, v128, q64, do64;
@@ -555,12 +638,12 @@ int launch_bwd(const AttnArgs& a, BwdParams p, float* neg_lse, float* delta, uin
 }
 
 template <int D, int FMT>
-int launch_variant(const AttnArgs& a, const BwdParams& p, float* neg_lse, float* delta, uint8_t* present, cudaStream_t st) {
+int launch_variant(const AttnArgs& a, const BwdParams& p, float* neg_lse, float* neg_delta, uint8_t* present, cudaStream_t st) {
   const bool drop = p.drop.threshold > 0;
-  if (a.mask) return drop ? launch_bwd<D, FMT, true, true>(a, p, neg_lse, delta, present, st)
-                          : launch_bwd<D, FMT, true, false>(a, p, neg_lse, delta, present, st);
-  return drop ? launch_bwd<D, FMT, false, true>(a, p, neg_lse, delta, present, st)
-              : launch_bwd<D, FMT, false, false>(a, p, neg_lse, delta, present, st);
+  if (a.mask) return drop ? launch_bwd<D, FMT, true, true>(a, p, neg_lse, neg_delta, present, st)
+                          : launch_bwd<D, FMT, true, false>(a, p, neg_lse, neg_delta, present, st);
+  return drop ? launch_bwd<D, FMT, false, true>(a, p, neg_lse, neg_delta, present, st)
+              : launch_bwd<D, FMT, false, false>(a, p, neg_lse, neg_delta, present, st);
 }
 
 int present_pitch(int Ns) { return (Ns / kBlk + 1) & ~1; }
@@ -578,20 +661,20 @@ int attn_bwd_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* statu
   BwdParams p = {};
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   float* neg_lse = reinterpret_cast<float*>(ws);
-  float* delta = reinterpret_cast<float*>(ws + stat_bytes(a.heads, a.Nt));
+  float* neg_delta = reinterpret_cast<float*>(ws + stat_bytes(a.heads, a.Nt));
   uint8_t* present = ws + 2 * stat_bytes(a.heads, a.Nt);
   p.row_ptr = a.row_ptr; p.idx = a.idx; p.mask = a.mask; p.present = present;
-  p.neg_lse = neg_lse; p.delta = delta;
+  p.neg_lse = neg_lse; p.neg_delta = neg_delta;
   p.Nt = a.Nt; p.Ns = a.Ns; p.heads = a.heads; p.kv_heads = a.kv_heads; p.group = a.heads / a.kv_heads;
   p.present_pitch = present_pitch(a.Ns);
   p.scale = a.scale; p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = status;
   p.drop = drop;
   if (a.D == 64)
-    return a.dtype == SPARTA_F16 ? launch_variant<64, 0>(a, p, neg_lse, delta, present, st)
-                                 : launch_variant<64, 1>(a, p, neg_lse, delta, present, st);
-  return a.dtype == SPARTA_F16 ? launch_variant<128, 0>(a, p, neg_lse, delta, present, st)
-                               : launch_variant<128, 1>(a, p, neg_lse, delta, present, st);
+    return a.dtype == SPARTA_F16 ? launch_variant<64, 0>(a, p, neg_lse, neg_delta, present, st)
+                                 : launch_variant<64, 1>(a, p, neg_lse, neg_delta, present, st);
+  return a.dtype == SPARTA_F16 ? launch_variant<128, 0>(a, p, neg_lse, neg_delta, present, st)
+                               : launch_variant<128, 1>(a, p, neg_lse, neg_delta, present, st);
 }
 
 }  // namespace sparta

@@ -270,12 +270,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     constexpr int kOChunks = D / 64;           // 32-column chunks of O per thread
     float m_run = -INFINITY, l_run = 0.f;
     PhiloxKey key = {};
-    uint32_t cut = 0;
     const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
-    if constexpr (DROP) {
-      key = load_philox_key(p.drop);
-      cut = p.drop.threshold << 16;
-    }
+    if constexpr (DROP) key = load_philox_key(p.drop);
     bool ok = true;
     for (int j = 0; j < npairs; ++j) {
       const int nblk = min(2, count - 2 * j);
@@ -373,20 +369,17 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         float sum = 0.f, sum1 = 0.f;
         auto exp_pack = [&](const uint32_t* v, uint32_t* out, int h) {  // scores 32 h .. -> 16 packed pairs (out may be v)
           uint32_t keep = 0;
-          if constexpr (DROP) keep = none ? 0u : philox_keep32(key, cut, kb * (kBlk / 32) + h, (uint32_t)grow, head);
+          if constexpr (DROP) keep = none ? 0u : philox_split32(key, p.drop.threshold, kb * (kBlk / 32) + h, (uint32_t)grow, head);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg_m));
-            float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg_m));
+            const float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg_m));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg_m));
             // the row sum takes the fp32 probabilities: their rounding to 16 bits for P V is unbiased, and
             // converting them back cost two instructions per pair in warps bound by instruction issue
             // (two alternating partial sums keep the additions from forming one dependent chain)
             if (i & 1) sum1 += p0 + p1; else sum += p0 + p1;
-            if constexpr (DROP) {
-              p0 = (keep >> (2 * i)) & 1u ? p0 : 0.f;
-              p1 = (keep >> (2 * i + 1)) & 1u ? p1 : 0.f;
-            }
             out[i] = pack2<T>(p0, p1);
+            if constexpr (DROP) out[i] &= pair_mask(keep, i);
           }
         };
         const uint32_t p_addr = tmem_base + lane_base + C::kPCol + colhalf * (kBlk / 2);

@@ -222,12 +222,8 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const long long grow = (long long)tile * kTileM + row;  // row inside the head
     float m_run = -INFINITY, l_run = 0.f;
     PhiloxKey key = {};
-    uint32_t cut = 0;
     const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
-    if constexpr (DROP) {
-      key = load_philox_key(p.drop);
-      cut = p.drop.threshold << 16;
-    }
+    if constexpr (DROP) key = load_philox_key(p.drop);
     bool ok = true;
     for (int j = 0; j < count; ++j) {
       const int e = ulist[j];
@@ -300,7 +296,7 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         uint32_t packed[16];
         if (mine) {
           uint32_t keep = 0;
-          if constexpr (DROP) keep = none ? 0u : philox_keep32(key, cut, kb * (kBlk / 32) + h, (uint32_t)grow, head);
+          if constexpr (DROP) keep = none ? 0u : philox_split32(key, p.drop.threshold, kb * (kBlk / 32) + h, (uint32_t)grow, head);
           if constexpr (!kHold) {
             tmem_ld_x32(s_addr + h * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
             tmem_ld_wait();
@@ -309,14 +305,11 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           const uint32_t* v = kHold ? &r[32 * h] : &r[0];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg_m));
-            float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg_m));
+            const float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg_m));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg_m));
             if (i & 1) sum1 += p0 + p1; else sum += p0 + p1;
-            if constexpr (DROP) {
-              p0 = (keep >> (2 * i)) & 1u ? p0 : 0.f;
-              p1 = (keep >> (2 * i + 1)) & 1u ? p1 : 0.f;
-            }
             packed[i] = pack2<T>(p0, p1);
+            if constexpr (DROP) packed[i] &= pair_mask(keep, i);
           }
         } else {
 #pragma unroll

@@ -78,12 +78,4 @@ __device__ __forceinline__ uint32_t philox_keep8(const PhiloxKey& key, uint32_t 
   return bits;
 }
 
-// the 32 decisions of columns 32 g .. 32 g + 31 of a row as one word
-__device__ __forceinline__ uint32_t philox_keep32(const PhiloxKey& key, uint32_t cut, uint32_t g, uint32_t row, uint32_t batch) {
-  uint32_t bits = 0;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) bits |= philox_keep8(key, cut, 4 * g + q, row, batch) << (8 * q);
-  return bits;
-}
-
 }  // namespace sparta
