@@ -103,7 +103,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 
   __shared__ float s_xchg[2][2][kTileM];  // [step parity][K block of the pair][row]: row maxima of the two threads of a row
   __shared__ float s_lsum[2][kTileM];     // their partial row sums, at the end
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the shuffles tell the compiler that the value is uniform over the warp: MMA descriptors then live in uniform registers
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // Launch order (see attn_tc2.cu): grouped by head when the K / V of all heads exceed L2, else head-major
   const int tiles_per_head = (p.Nt + kTileM - 1) / kTileM;  // the last tile may be one block row high
   int head, tile;
@@ -162,8 +163,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_holder;
-  const int count = *s_count;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
+  const int count = __shfl_sync(0xffffffffu, *s_count, 0);
   const int npairs = (count + 1) / 2;
   const long long q_row0 = (long long)head * p.Nt + (long long)tile * kTileM;
   const long long kv_row0 = (long long)(head / p.group) * p.Ns;
@@ -203,14 +204,14 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     // ------------------------------ S = Q K^T ------------------------------
     const uint64_t desc_hi = make_smem_desc(0, 16, 1024, SW_128B);
     const uint32_t q_lo = smem_u32(q_s) >> 4, k_lo = smem_u32(k_s) >> 4;
-    bool ok = count == 0 || mbar_wait(q_full, 0);
+    bool ok = count == 0 || mbar_wait_warp(q_full, 0);
     for (int j = 0; j < npairs && ok; ++j) {
       const int nblk = min(2, count - 2 * j);
       const int ks = j % kKStages, sb = j % kSBuf;
-      if (!mbar_wait(&k_full[ks], (j / kKStages) & 1)) { ok = false; break; }
-      if (!mbar_wait(&s_empty[sb], ((j / kSBuf) & 1) ^ 1)) { ok = false; break; }
+      if (!mbar_wait_warp(&k_full[ks], (j / kKStages) & 1)) { ok = false; break; }
+      if (!mbar_wait_warp(&s_empty[sb], ((j / kSBuf) & 1) ^ 1)) { ok = false; break; }
       tc_fence_after_sync();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t idesc = make_idesc_f16(kTileM, nblk * kBlk, FMT, 0, 0);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -237,10 +238,10 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     for (int j = 0; j < npairs && ok; ++j) {
       const int nblk = min(2, count - 2 * j);
       const int vs = j % kVStages;
-      if (!mbar_wait(&v_full[vs], (j / kVStages) & 1)) { ok = false; break; }
-      if (!mbar_wait(p_full, j & 1)) { ok = false; break; }
+      if (!mbar_wait_warp(&v_full[vs], (j / kVStages) & 1)) { ok = false; break; }
+      if (!mbar_wait_warp(p_full, j & 1)) { ok = false; break; }
       tc_fence_after_sync();
-      if (lane == 0) {
+      if (elect_one()) {
         for (int kk = 0; kk < nblk * (kBlk / 16); ++kk) {
           const uint32_t b_off = (vs * C::kKVBytes + kk * 16 * 128) >> 4;
           umma_ts(tmem_base + C::kOCol, tmem_base + C::kPCol + kk * 8, v_desc_hi | (v_lo + b_off), idesc,

@@ -128,7 +128,8 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 
   __shared__ float s_xchg[kTiles][2][2][kTileM];  // [tile][step parity][K block of the pair][row]: row maxima of the two threads of a row
   __shared__ float s_lsum[kTiles][2][kTileM];     // their partial row sums, at the end
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the shuffles tell the compiler that the value is uniform over the warp: MMA descriptors then live in uniform registers
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   TR_DECL;
   TR_T0(t_cta);
   // Launch order.  grouped: first the first tile of every head (with a global-token row it is the heaviest by
@@ -197,8 +198,8 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_holder;
-  const int count = *s_count;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
+  const int count = __shfl_sync(0xffffffffu, *s_count, 0);
   const int npairs = (count + 1) / 2;
   const long long q_row0 = (long long)head * p.Nt + (long long)cta_tile * (kTiles * kTileM);
   const long long kv_row0 = (long long)(head / p.group) * p.Ns;
@@ -274,7 +275,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const uint32_t t_base0 = tmem_base, t_base1 = tmem_base + C::kTileCols;
     constexpr uint32_t idesc_pv = make_idesc_f16(kTileM, D, FMT, 0, 1);
     constexpr uint32_t idesc_qk2 = make_idesc_f16(kTileM, 2 * kBlk, FMT, 0, 0), idesc_qk1 = make_idesc_f16(kTileM, kBlk, FMT, 0, 0);
-    bool ok = count == 0 || mbar_wait(q_full, 0);
+    bool ok = count == 0 || mbar_wait_warp(q_full, 0);
     int taken[kTiles] = {0, 0};  // P.V steps issued per tile
     // last step each tile takes part in: only there does its epilogue need "P.V complete"
     int last_step[kTiles] = {-1, -1};
@@ -286,7 +287,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     // scores of a step for tile t from K stage st (both indexes select registers), then "scores complete"
     auto issue_qk = [&](int t, int st, int nblk) {
       tc_fence_after_sync();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t qb = t ? q_base1 : q_base0, kb = st ? k_base1 : k_base0, d = t ? t_base1 : t_base0;
         const uint32_t idesc = nblk == 2 ? idesc_qk2 : idesc_qk1;
 #pragma unroll
@@ -300,7 +301,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     };
     auto issue_pv = [&](int t, int st, int nblk, bool first, bool last) {
       tc_fence_after_sync();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t vb = st ? v_base1 : v_base0, tb = t ? t_base1 : t_base0;
 #pragma unroll
         for (int kk = 0; kk < 2 * (kBlk / 16); ++kk) {
@@ -316,13 +317,13 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     uint32_t bits_next = npairs > 0 ? step_bits(0) : 0u;
     if (ok && npairs > 0) {
       TR_T0(t_kf);
-      ok = mbar_wait(&k_full[0], 0);
+      ok = mbar_wait_warp(&k_full[0], 0);
       TR_ADD(1, t_kf);
       if (ok) {
         const int nblk0 = min(2, count);
         if (bits_next & 3u) issue_qk(0, 0, nblk0);
         if (bits_next & 12u) issue_qk(1, 0, nblk0);
-        if (lane == 0) umma_commit(&k_empty[0]);
+        if (elect_one()) umma_commit(&k_empty[0]);
         __syncwarp();
       }
     }
@@ -334,7 +335,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       bits_next = more ? step_bits(j + 1) : 0u;
       const int nblk_next = min(2, count - 2 * (j + 1));
       TR_T0(t_vf);
-      if (!mbar_wait(&v_full[st], (j / kStages) & 1)) { ok = false; break; }
+      if (!mbar_wait_warp(&v_full[st], (j / kStages) & 1)) { ok = false; break; }
       TR_ADD(3, t_vf);
       bool k_ready = false;
 #pragma unroll
@@ -342,7 +343,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         if (!ok) break;
         if ((bits >> (2 * t)) & 3u) {
           TR_T0(t_pf);
-          if (!mbar_wait(&p_full[t], taken[t] & 1)) { ok = false; break; }
+          if (!mbar_wait_warp(&p_full[t], taken[t] & 1)) { ok = false; break; }
           TR_ADD(4, t_pf);
           issue_pv(t, st, nblk, taken[t] == 0, j == last_step[t]);
           ++taken[t];
@@ -350,7 +351,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         if ((bits_next >> (2 * t)) & 3u) {
           if (!k_ready) {
             TR_T0(t_kf);
-            if (!mbar_wait(&k_full[st_next], ((j + 1) / kStages) & 1)) { ok = false; break; }
+            if (!mbar_wait_warp(&k_full[st_next], ((j + 1) / kStages) & 1)) { ok = false; break; }
             TR_ADD(1, t_kf);
             k_ready = true;
           }
@@ -358,7 +359,7 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         }
       }
       if (!ok) break;
-      if (lane == 0) {
+      if (elect_one()) {
         umma_commit(&v_empty[st]);
         if (more) umma_commit(&k_empty[st_next]);
       }

@@ -81,7 +81,8 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   int* s_count = reinterpret_cast<int*>(tmem_holder + 1);
   int* s_range = s_count + 1;             // [2]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the shuffles tell the compiler that the value is uniform over the warp: MMA descriptors then live in uniform registers
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int tiles_per_head = (p.Nt + kTileM - 1) / kTileM;  // the last tile may be one block row high
   int head, tile;
   if (!p.grouped) {
@@ -141,8 +142,8 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem_base = *tmem_holder;
-  const int count = *s_count;  // steps
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
+  const int count = __shfl_sync(0xffffffffu, *s_count, 0);  // steps
   const long long q_row0 = (long long)head * p.Nt + (long long)tile * kTileM;
   const long long kv_row0 = (long long)(head / p.group) * p.Ns;
 
@@ -179,7 +180,7 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     constexpr uint32_t idesc_pv = make_idesc_f16(kTileM, kD, FMT, 0, 1);
     auto issue_qk = [&](int st) {
       tc_fence_after_sync();
-      if (lane == 0) {
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kD / 16; ++kk)
           umma_ss(tmem_base, desc_hi | (q_lo + 2 * kk), desc_hi | (k_lo + ((st * kKVBytes) >> 4) + 2 * kk), idesc_qk,
@@ -189,14 +190,14 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       }
       __syncwarp();
     };
-    bool ok = count == 0 || (mbar_wait(q_full, 0) && mbar_wait(&k_full[0], 0));
+    bool ok = count == 0 || (mbar_wait_warp(q_full, 0) && mbar_wait_warp(&k_full[0], 0));
     if (ok && count > 0) issue_qk(0);
     for (int j = 0; j < count && ok; ++j) {
       const int st = j % kStages;
-      if (!mbar_wait(&v_full[st], (j / kStages) & 1)) { ok = false; break; }
-      if (!mbar_wait(p_full, j & 1)) { ok = false; break; }
+      if (!mbar_wait_warp(&v_full[st], (j / kStages) & 1)) { ok = false; break; }
+      if (!mbar_wait_warp(p_full, j & 1)) { ok = false; break; }
       tc_fence_after_sync();
-      if (lane == 0) {
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kBlk / 16; ++kk)
           umma_ts(tmem_base + kOCol, tmem_base + kk * 8, v_desc_hi | (v_lo + ((st * kKVBytes + kk * 16 * 128) >> 4)),
@@ -207,7 +208,7 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       __syncwarp();
       if (j + 1 < count) {
         const int sn = (j + 1) % kStages;
-        if (!mbar_wait(&k_full[sn], ((j + 1) / kStages) & 1)) { ok = false; break; }
+        if (!mbar_wait_warp(&k_full[sn], ((j + 1) / kStages) & 1)) { ok = false; break; }
         issue_qk(sn);
       }
     }
