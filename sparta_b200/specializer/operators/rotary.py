@@ -1,9 +1,8 @@
 """``RotaryEmbedding``: rotary positions on queries and keys (``sparta_rotary``).  The reference's attention knows no
 positions; the layer around it turns queries and keys before it calls the operator."""
-import ctypes
 import math
 from decimal import Decimal, localcontext
-from typing import Dict, List, Optional, Tuple, Union
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -44,57 +43,60 @@ def as_turns(freq: List[float]) -> List[int]:
     return [w - (1 << 64) if w >= 1 << 63 else w for w in whole]
 
 
-class _View(object):
-    """A tensor (..., N, E) as [batch, heads, n, dim] with strides, next to its positions."""
-
-    __slots__ = ('x', 'batch', 'heads', 'n', 'strides', 'positions', 'per_batch')
-
-    def __init__(self, x: torch.Tensor, positions: Optional[torch.Tensor]):
-        if x.dim() > 4:
-            x = x.flatten(0, -3)
-        if x.stride(-1) != 1:
-            x = x.contiguous()
-        n = x.shape[-2]
-        rows = positions.shape[0] if positions is not None and positions.dim() == 2 else 1
-        s = x.stride()
-        if x.dim() == 4:
-            self.batch, self.heads, self.strides = x.shape[0], x.shape[1], s[:3]
-            if rows not in (1, self.batch):
-                raise ValueError(f'positions of {rows} sequences for a batch of {self.batch}')
-        elif x.dim() == 3:
-            if x.shape[0] % rows:
-                raise ValueError(f'positions of {rows} sequences for {x.shape[0]} heads')
-            self.batch, self.heads = rows, x.shape[0] // rows
-            self.strides = (self.heads * s[0], s[0], s[1])
-        else:
-            if rows != 1:
-                raise ValueError(f'positions of {rows} sequences for one')
-            self.batch, self.heads, self.strides = 1, 1, (0, 0, s[0])
-        if positions is not None and positions.shape[-1] != n:
+def _record(x: torch.Tensor, y: torch.Tensor, positions: Optional[torch.Tensor]):
+    """(tensor to keep alive, ``sparta_rotary_tensor``): (..., N, E) as [batch, heads, n, dim] with strides, next to its
+    positions."""
+    if x.dim() > 4:
+        x = x.flatten(0, -3)
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    shape, s = x.shape, x.stride()
+    n, rows, pos = shape[-2], 1, None
+    if positions is not None:
+        pos = positions.data_ptr()
+        if positions.dim() == 2:
+            rows = positions.shape[0]
+        if positions.shape[-1] != n:
             raise ValueError(f'{positions.shape[-1]} positions for {n} tokens')
-        self.x, self.n, self.positions, self.per_batch = x, n, positions, int(rows > 1)
+    if len(shape) == 4:
+        batch, heads = shape[0], shape[1]
+        if rows != 1 and rows != batch:
+            raise ValueError(f'positions of {rows} sequences for a batch of {batch}')
+        sb, sh, sn = s[0], s[1], s[2]
+    elif len(shape) == 3:
+        if shape[0] % rows:
+            raise ValueError(f'positions of {rows} sequences for {shape[0]} heads')
+        batch, heads = rows, shape[0] // rows
+        sb, sh, sn = heads * s[0], s[0], s[1]
+    else:
+        if rows != 1:
+            raise ValueError(f'positions of {rows} sequences for one')
+        batch, heads, sb, sh, sn = 1, 1, 0, 0, s[0]
+    return x, _lib.RotaryTensor(x.data_ptr(), y.data_ptr(), pos, sb, sh, sn, batch, heads, n, 1 if rows > 1 else 0)
 
 
-def _launch(module: 'RotaryEmbedding', tensors: List[torch.Tensor], positions: List[Optional[torch.Tensor]],
+_Two = _lib.RotaryTensor * 2
+
+
+def _launch(module: 'RotaryEmbedding', tensors: Sequence[torch.Tensor], positions: Sequence[Optional[torch.Tensor]],
             backward: bool) -> List[torch.Tensor]:
-    outs, records, keep = [], [], []
+    outs, records, keep, wide = [], [], [], 0
     for x, pos in zip(tensors, positions):
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         outs.append(y)
-        if x.numel() == 0:
-            continue
-        v = _View(x.detach(), pos)
-        keep.append(v)
-        records.append(_lib.RotaryTensor(v.x.data_ptr(), y.data_ptr(), _lib.ptr(pos), *v.strides, v.batch, v.heads, v.n,
-                                         v.per_batch))
+        if x.numel() > 0:
+            held, record = _record(x, y, pos)
+            keep.append(held)
+            records.append(record)
+            if pos is not None:
+                wide = pos.dtype == torch.int64
     if records:
-        x = keep[0].x
-        given = [v.positions for v in keep if v.positions is not None]
-        with _lib.on_device(x.device):
+        x = keep[0]
+        device = x.device
+        with _lib.on_device(device):
             _lib.check(_lib.lib().sparta_rotary(
-                (_lib.RotaryTensor * len(records))(*records), len(records), module._turns(x.device).data_ptr(),
-                module.head_dim, module.rotary_dim, int(module.interleaved), module.magnitude, int(backward),
-                int(bool(given) and given[0].dtype == torch.int64), _lib.dtype_code(x), _lib.stream_ptr(x.device)),
+                _Two(*records), len(records), module._turns(device).data_ptr(), module.head_dim, module.rotary_dim,
+                module.interleaved, module.magnitude, backward, wide, _lib.dtype_code(x), _lib.stream_ptr(device)),
                 'sparta_rotary')
     return outs
 
@@ -106,7 +108,7 @@ class RotaryFunc(torch.autograd.Function):
         ctx.module, ctx.reverse = module, not backward
         ctx.save_for_backward(query_positions, key_positions)
         ctx.set_materialize_grads(False)
-        return tuple(_launch(module, list(tensors), [query_positions, key_positions][:len(tensors)], backward))
+        return tuple(_launch(module, tensors, (query_positions, key_positions), backward))
 
     @staticmethod
     def backward(ctx, *grads):
@@ -114,8 +116,10 @@ class RotaryFunc(torch.autograd.Function):
         wanted = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[4 + i]]
         out: List[Optional[torch.Tensor]] = [None] * len(grads)
         if wanted:
-            pos = [positions[i] for i in wanted] + [None]
-            turned = RotaryFunc.apply(ctx.module, ctx.reverse, pos[0], pos[1], *[grads[i] for i in wanted])
+            pos, given = [positions[i] for i in wanted] + [None], [grads[i] for i in wanted]
+            # linear: the gradient's own gradient is the same operator; the plain launch skips autograd's bookkeeping
+            turned = (RotaryFunc.apply(ctx.module, ctx.reverse, pos[0], pos[1], *given) if torch.is_grad_enabled()
+                      else _launch(ctx.module, given, pos, ctx.reverse))
             for i, g in zip(wanted, turned):
                 out[i] = g
         return (None, None, None, None, *out)
@@ -152,7 +156,7 @@ class RotaryEmbedding(torch.nn.Module):
             raise ValueError('base and factor have to be positive numbers')
         if scaling == 'yarn' and not (original_length and original_length > 0):
             raise ValueError("scaling 'yarn' needs original_length")
-        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, bool(interleaved)
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, int(bool(interleaved))
         self.scaling, self.factor, self.base, self.original_length = scaling, factor, base, original_length
         freq, self.magnitude = rotary_frequencies(rotary_dim, base, scaling, factor, original_length)
         self._turn_list = as_turns(freq)
@@ -180,16 +184,19 @@ class RotaryEmbedding(torch.nn.Module):
                 key_positions: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
         if key is not None and key_positions is None:
             key_positions = positions
-        if key_positions is not None and positions is not None and key_positions.dtype != positions.dtype:
+        if key_positions is not positions and key_positions is not None and positions is not None \
+                and key_positions.dtype != positions.dtype:
             positions, key_positions = positions.long(), key_positions.long()
-        positions = positions if positions is None else positions.contiguous()
         self._check(query, positions, query)
+        if positions is not None:
+            positions = positions.contiguous()
         if key is None:
             return RotaryFunc.apply(self, False, positions, None, query)[0]
-        key_positions = key_positions if key_positions is None else key_positions.contiguous()
         self._check(key, key_positions, query)
+        if key_positions is not None:
+            key_positions = key_positions.contiguous()
         return RotaryFunc.apply(self, False, positions, key_positions, query, key)
 
     def extra_repr(self) -> str:
         return (f'head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, base={self.base}, '
-                f'interleaved={self.interleaved}, scaling={self.scaling!r}')
+                f'interleaved={bool(self.interleaved)}, scaling={self.scaling!r}')

@@ -163,12 +163,11 @@ class SparseAttention(OperatorBase):
     def _train_args(self, q, k, v, out, lse, indexes, mask, p: float, numbers: DropoutKey) -> '_lib.AttnTrainArgs':
         if self._attn_status is None or self._attn_status.device != q.device:
             self._attn_status = torch.zeros(4, dtype=torch.int32, device=q.device)
-        return _lib.AttnTrainArgs(
-            Q=q.data_ptr(), K=k.data_ptr(), V=v.data_ptr(), O=out.data_ptr(), lse=lse.data_ptr(),
-            row_ptr=indexes.row_ptr.data_ptr(), bcsr_idx=indexes.bcsr_buf.data_ptr(), mask=_lib.ptr(mask),
-            rng=_lib.ptr(numbers.rng), seed=numbers.seed & 0xffffffffffffffff, call=numbers.call & 0xffffffff,
-            status=self._attn_status.data_ptr(), dropout=p, scale=self._scale, heads=q.shape[0], kv_heads=k.shape[0],
-            Nt=self._Nt, Ns=self._Ns, D=q.shape[2], BLK=FUSED_BLOCK, dtype=_lib.dtype_code(q))
+        return _lib.AttnTrainArgs(  # in the order of its fields
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), None, None, None, None, None, 0,
+            indexes.row_ptr.data_ptr(), indexes.bcsr_buf.data_ptr(), _lib.ptr(mask), _lib.ptr(numbers.rng),
+            numbers.seed & 0xffffffffffffffff, numbers.call & 0xffffffff, self._attn_status.data_ptr(), p, self._scale,
+            q.shape[0], k.shape[0], self._Nt, self._Ns, q.shape[2], FUSED_BLOCK, _lib.dtype_code(q))
 
     def _raise_on_status(self):
         if self.check_status and any(self.fused_status()):

@@ -49,24 +49,27 @@ class _Counter(object):
         return key
 
 
-def _launch(x: torch.Tensor, p: float, key: DropoutKey, indexes: Optional[BCSIndexes]) -> torch.Tensor:
+def _launch(x: torch.Tensor, p: float, rng: Optional[torch.Tensor], seed: int, call: int,
+            indexes: Optional[BCSIndexes]) -> torch.Tensor:
     x = x.contiguous()
     y = torch.empty_like(x)
-    if x.numel() == 0:
+    n = x.numel()
+    if n == 0:
         return y
-    tail = (float(p), _lib.ptr(key.rng), key.seed & 0xffffffffffffffff, key.call & 0xffffffff, _lib.dtype_code(x))
-    with _lib.on_device(x.device):
-        stream = _lib.stream_ptr(x.device)
+    device, shape = x.device, x.shape
+    with _lib.on_device(device):
         if indexes is None:
-            W = x.shape[-1] if x.dim() > 0 else 1
-            H = x.shape[-2] if x.dim() > 1 else 1
-            _lib.check(_lib.lib().sparta_dropout(x.data_ptr(), y.data_ptr(), x.numel() // (H * W), H, W, *tail, stream),
-                       'sparta_dropout')
+            W = shape[-1] if shape else 1
+            H = shape[-2] if len(shape) > 1 else 1
+            _lib.check(_lib.lib().sparta_dropout(
+                x.data_ptr(), y.data_ptr(), n // (H * W), H, W, p, _lib.ptr(rng), seed & 0xffffffffffffffff,
+                call & 0xffffffff, _lib.dtype_code(x), _lib.stream_ptr(device)), 'sparta_dropout')
         else:
-            stride = indexes.val_stride_blocks
             _lib.check(_lib.lib().sparta_dropout_blocks(
-                x.data_ptr(), y.data_ptr(), indexes.bcsr_buf.data_ptr(), indexes.nnz_dev.data_ptr(),
-                x.numel() // x.shape[-1], indexes.block_H, indexes.block_W, stride, *tail, stream), 'sparta_dropout_blocks')
+                x.data_ptr(), y.data_ptr(), indexes.bcsr_buf.data_ptr(), indexes.nnz_dev.data_ptr(), n // shape[-1],
+                indexes.block_H, indexes.block_W, indexes.val_stride_blocks, p, _lib.ptr(rng),
+                seed & 0xffffffffffffffff, call & 0xffffffff, _lib.dtype_code(x), _lib.stream_ptr(device)),
+                'sparta_dropout_blocks')
     return y
 
 
@@ -77,12 +80,14 @@ class SparseDropoutFunc(torch.autograd.Function):
                 indexes: Optional[BCSIndexes]):
         ctx.p, ctx.numbers, ctx.indexes = p, (seed, call), indexes
         ctx.save_for_backward(rng)  # rewritten before the backward pass: autograd refuses
-        return _launch(x.detach(), p, DropoutKey(rng, seed, call), indexes)
+        return _launch(x, p, rng, seed, call, indexes)
 
     @staticmethod
     def backward(ctx, grad: torch.Tensor):
         rng, = ctx.saved_tensors
-        return SparseDropoutFunc.apply(grad, ctx.p, rng, *ctx.numbers, ctx.indexes), None, None, None, None, None
+        # linear: the gradient's own gradient is the same operator; the plain launch skips autograd's bookkeeping
+        run = SparseDropoutFunc.apply if torch.is_grad_enabled() else _launch
+        return run(grad, ctx.p, rng, *ctx.numbers, ctx.indexes), None, None, None, None, None
 
 
 def sparse_dropout(x: torch.Tensor, p: float, key: DropoutKey, indexes: Optional[BCSIndexes] = None) -> torch.Tensor:
