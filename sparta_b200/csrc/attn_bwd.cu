@@ -432,15 +432,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
       nd.x = nd.y = __ldg(p.neg_delta + a_row0 + row);
     }
     PhiloxKey key = {};
-    const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
-    if constexpr (DROP) key = load_philox_key(p.drop);
+    PhiloxRow key_row = {};
+    if constexpr (DROP) {
+      key = load_uniform_philox_key(p.drop);
+      if constexpr (!DKV) key_row = philox_row(key, grow, head);
+    }
+    const uint32_t t2 = threshold2(p.drop);
     const float up = p.drop.scale;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     int h = 0, k = 0;  // step = h * pairs + k
     for (int j = 0; j < steps; ++j) {
       const int st = j % kStages, at = C::kBlocks * k + (quarter >> 1);
-      const int e = at < count ? ulist[at] : 0;
+      const int e = __shfl_sync(0xffffffffu, at < count ? ulist[at] : 0, 0);
       const bool there = at < count;                   // the pair has this block
       const bool mine = (e >> half) & 1;               // it is kept for this warp's rows
       const int blk = e >> 2;
@@ -457,7 +461,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
         }
         if constexpr (DROP) {
           const int q_head = DKV ? head * p.group + h : head;
-          keep_w = none ? 0u : philox_split32(key, p.drop.threshold, word, q_row, q_head);
+          if constexpr (DKV) key_row = philox_row(key, q_row, q_head);
+          keep_w = philox_split32(key, key_row, t2, word, q_head);
           if constexpr (DKV) keep_w = __shfl_sync(0xffffffffu, transpose_bits32(keep_w, lane), to_split32(lane));
         }
       }

@@ -271,8 +271,12 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     constexpr int kOChunks = D / 64;           // 32-column chunks of O per thread
     float m_run = -INFINITY, l_run = 0.f;
     PhiloxKey key = {};
-    const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
-    if constexpr (DROP) key = load_philox_key(p.drop);
+    PhiloxRow key_row = {};
+    if constexpr (DROP) {
+      key = load_uniform_philox_key(p.drop);
+      key_row = philox_row(key, (uint32_t)grow, head);
+    }
+    const uint32_t t2 = threshold2(p.drop);
     bool ok = true;
     for (int j = 0; j < npairs; ++j) {
       const int nblk = min(2, count - 2 * j);
@@ -369,8 +373,6 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         const float neg_m = m_run > -INFINITY ? -m_run : -INFINITY;
         float sum = 0.f, sum1 = 0.f;
         auto exp_pack = [&](const uint32_t* v, uint32_t* out, int h) {  // scores 32 h .. -> 16 packed pairs (out may be v)
-          uint32_t keep = 0;
-          if constexpr (DROP) keep = none ? 0u : philox_split32(key, p.drop.threshold, kb * (kBlk / 32) + h, (uint32_t)grow, head);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * i]), p.scale_log2, neg_m));
@@ -380,8 +382,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             // (two alternating partial sums keep the additions from forming one dependent chain)
             if (i & 1) sum1 += p0 + p1; else sum += p0 + p1;
             out[i] = pack2<T>(p0, p1);
-            if constexpr (DROP) out[i] &= pair_mask(keep, i);
           }
+          if constexpr (DROP) drop_packed32(out, key, key_row, t2, kb * (kBlk / 32) + h, head);
         };
         const uint32_t p_addr = tmem_base + lane_base + C::kPCol + colhalf * (kBlk / 2);
         if constexpr (kHold) {

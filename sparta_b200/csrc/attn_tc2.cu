@@ -386,8 +386,12 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     constexpr int kOChunks = D / 64;           // 32-column chunks of O per thread
     float m_run = -INFINITY, l_run = 0.f;
     PhiloxKey key = {};
-    const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
-    if constexpr (DROP) key = load_philox_key(p.drop);
+    PhiloxRow key_row = {};
+    if constexpr (DROP) {
+      key = load_uniform_philox_key(p.drop);
+      key_row = philox_row(key, (uint32_t)grow, head);
+    }
+    const uint32_t t2 = threshold2(p.drop);
     bool ok = true;
     int taken = 0;
     for (int j = 0; j < npairs; ++j) {
@@ -480,8 +484,6 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           for (int h = 0; h < 2; ++h) {
             uint32_t packed[16];
             if (mine) {
-              uint32_t keep = 0;
-              if constexpr (DROP) keep = none ? 0u : philox_split32(key, p.drop.threshold, kb * (kBlk / 32) + h, (uint32_t)grow, head);
               tmem_ld_x32(s_addr + h * 32, r);
               tmem_ld_wait();
               if (p.mask) mask_scores(r, h);
@@ -493,8 +495,8 @@ attn_fwd_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 // alternating partial sums keep the additions from forming one dependent chain
                 if (i & 1) sum1 += p0 + p1; else sum += p0 + p1;
                 packed[i] = pack2<T>(p0, p1);
-                if constexpr (DROP) packed[i] &= pair_mask(keep, i);
               }
+              if constexpr (DROP) drop_packed32(packed, key, key_row, t2, kb * (kBlk / 32) + h, head);
             } else {
 #pragma unroll
               for (int i = 0; i < 16; ++i) packed[i] = 0;

@@ -223,8 +223,12 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const long long grow = (long long)tile * kTileM + row;  // row inside the head
     float m_run = -INFINITY, l_run = 0.f;
     PhiloxKey key = {};
-    const bool none = DROP && p.drop.threshold >= kDropoutOne;  // everything dropped
-    if constexpr (DROP) key = load_philox_key(p.drop);
+    PhiloxRow key_row = {};
+    if constexpr (DROP) {
+      key = load_uniform_philox_key(p.drop);
+      key_row = philox_row(key, (uint32_t)grow, head);
+    }
+    const uint32_t t2 = threshold2(p.drop);
     bool ok = true;
     for (int j = 0; j < count; ++j) {
       const int e = ulist[j];
@@ -296,8 +300,6 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       for (int h = 0; h < 2; ++h) {
         uint32_t packed[16];
         if (mine) {
-          uint32_t keep = 0;
-          if constexpr (DROP) keep = none ? 0u : philox_split32(key, p.drop.threshold, kb * (kBlk / 32) + h, (uint32_t)grow, head);
           if constexpr (!kHold) {
             tmem_ld_x32(s_addr + h * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
             tmem_ld_wait();
@@ -310,8 +312,8 @@ attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             const float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * i + 1]), p.scale_log2, neg_m));
             if (i & 1) sum1 += p0 + p1; else sum += p0 + p1;
             packed[i] = pack2<T>(p0, p1);
-            if constexpr (DROP) packed[i] &= pair_mask(keep, i);
           }
+          if constexpr (DROP) drop_packed32(packed, key, key_row, t2, kb * (kBlk / 32) + h, head);
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) packed[i] = 0;
