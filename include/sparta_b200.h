@@ -254,7 +254,8 @@ int sparta_attn_fwd_gather(const void* Q, const void* K, const void* V, void* O,
  *   pass, which needs the forward's O, mask, indexes and random numbers again.  dQ may be NULL, and so may dK and dV
  *   together: what is not wanted is not computed.
  *   dropout in [0, 1], rng / seed / call as for sparta_dropout.
- *   workspace (backward only): sparta_attn_train_bwd_workspace_bytes(), 16-byte aligned, no initial contents.
+ *   nnz_hint: kept blocks of the mask as far as the host knows (0: unknown); decides only how the backward pass divides
+ *   its work over the GPU.  workspace (backward only): sparta_attn_train_bwd_workspace_bytes(), 16-byte aligned, no initial contents.
  */
 typedef struct sparta_attn_train_args {
   const void* Q;
@@ -273,6 +274,7 @@ typedef struct sparta_attn_train_args {
   const uint8_t* mask;
   const int64_t* rng;
   uint64_t seed, call;
+  int64_t nnz_hint;
   int32_t* status;
   double dropout;
   float scale;
@@ -281,7 +283,7 @@ typedef struct sparta_attn_train_args {
 
 int sparta_attn_train_fwd(const sparta_attn_train_args* h_args, void* stream);
 
-size_t sparta_attn_train_bwd_workspace_bytes(int heads, int Nt, int Ns);
+size_t sparta_attn_train_bwd_workspace_bytes(int heads, int kv_heads, int Nt, int Ns, int D, int64_t nnz_hint);
 
 int sparta_attn_train_bwd(const sparta_attn_train_args* h_args, void* stream);
 

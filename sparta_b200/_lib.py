@@ -51,7 +51,7 @@ class AttnTrainArgs(ctypes.Structure):
         ('dO', c_void_p), ('dQ', c_void_p), ('dK', c_void_p), ('dV', c_void_p),
         ('workspace', c_void_p), ('workspace_bytes', c_size_t),
         ('row_ptr', c_void_p), ('bcsr_idx', c_void_p), ('mask', c_void_p), ('rng', c_void_p),
-        ('seed', c_uint64), ('call', c_uint64), ('status', c_void_p), ('dropout', c_double), ('scale', c_float),
+        ('seed', c_uint64), ('call', c_uint64), ('nnz_hint', c_int64), ('status', c_void_p), ('dropout', c_double), ('scale', c_float),
         ('heads', c_int32), ('kv_heads', c_int32), ('Nt', c_int32), ('Ns', c_int32), ('D', c_int32), ('BLK', c_int32),
         ('dtype', c_int32),
     ]
@@ -100,7 +100,7 @@ SIGNATURES = {
                                        c_void_p, c_float, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
                                        c_void_p, POINTER(c_void_p), c_int, c_void_p]),
     'sparta_attn_train_fwd': (c_int, [POINTER(AttnTrainArgs), c_void_p]),
-    'sparta_attn_train_bwd_workspace_bytes': (c_size_t, [c_int] * 3),
+    'sparta_attn_train_bwd_workspace_bytes': (c_size_t, [c_int] * 5 + [c_int64]),
     'sparta_attn_train_bwd': (c_int, [POINTER(AttnTrainArgs), c_void_p]),
     'sparta_dropout': (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_double, c_void_p, c_uint64, c_uint64,
                                c_int, c_void_p]),

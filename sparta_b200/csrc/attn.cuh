@@ -24,6 +24,7 @@ struct AttnArgs {
   float scale;
   int heads, kv_heads;      // heads / kv_heads query heads share a key / value head
   int Nt, Ns, D, dtype;
+  long long nnz;            // kept blocks, 0 when unknown
 };
 
 // fused attention with two Q tiles per CTA (attn_tc2.cu): query lengths that are a multiple of 256
@@ -36,7 +37,7 @@ int attn_tc2_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* statu
 int attn_tc64_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* status, cudaStream_t st);
 
 // backward pass (attn_bwd.cu)
-size_t attn_bwd_workspace(int heads, int Nt, int Ns);
+size_t attn_bwd_workspace(int heads, int kv_heads, int Nt, int Ns, int D, long long nnz);
 int attn_bwd_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* status, cudaStream_t st);
 
 // 2^x by the special-function unit alone.  exp2f() wraps the same instruction in a range fix for

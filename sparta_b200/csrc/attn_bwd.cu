@@ -7,7 +7,7 @@
 //   dS = P (dP - delta)      dQ = scale dS K       dK = scale dS^T Q        (K, V shared by heads: summed over them)
 //
 // Two passes over the kept blocks, each with its sums in tensor memory from the first block to the last, so that every
-// gradient is written once, in a fixed order of additions, without atomics and without a 32-bit workspace: one pass
+// gradient is written once, in a fixed order of additions: one pass
 // owns 128 query rows and walks the kept key blocks (dQ), the other owns 128 key rows and walks the query blocks of
 // every head that shares them (dK, dV).  That is seven products per kept block instead of the five of a single pass,
 // which would have to add 128 x D 32-bit partial sums of dQ per block to global memory (in an order that changes from
@@ -65,6 +65,10 @@ struct BwdParams {
   int Nt, Ns, heads, kv_heads, group;
   int present_pitch;
   int by_head;              // launch order: tiles of a head together
+  int split;                // CTAs per tile at most, see the kernel
+  int split_steps;          // steps that one of them should take
+  float* partial;           // [heads, tiles, split, 128, columns of the sums], where a tile is split
+  uint32_t* tickets;        // [heads, tiles], zero
   float scale, scale_log2;
   int32_t* status;
   DropoutParams drop;
@@ -126,7 +130,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256)
 attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const float* __restrict__ lse, float* __restrict__ neg_lse,
                      float* __restrict__ neg_delta, uint8_t* __restrict__ present, const int32_t* __restrict__ row_ptr,
-                     const int32_t* __restrict__ idx, long long rows, int nbr, int nbc, int pitch) {
+                     const int32_t* __restrict__ idx, long long rows, int nbr, int nbc, int pitch,
+                     uint32_t* __restrict__ tickets, long long n_tickets) {
   constexpr int kLanes = D / 8;
   const int lane = threadIdx.x % kLanes;
   const long long row = (long long)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
@@ -145,6 +150,7 @@ attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const fl
     neg_delta[row] = -sum;
     neg_lse[row] = lse[row] > -INFINITY ? lse[row] * -1.4426950408889634f : -INFINITY;
   }
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n_tickets; i += (long long)gridDim.x * 256) tickets[i] = 0;
   __shared__ uint8_t kept[kMaxBlocks];
   for (int r = blockIdx.x; r < nbr; r += gridDim.x) {  // block rows of the mask
     __syncthreads();
@@ -159,7 +165,9 @@ attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const fl
   }
 }
 
-template <bool DKV, int D, int FMT, bool MASK, bool DROP>
+// SPLIT: several CTAs may share a tile.  A variant of its own, because the other one keeps its registers for the steps
+// (B4 H16 S4096 D64, which does not split: 509 us with the code for it, 483 us without).
+template <bool DKV, int D, int FMT, bool MASK, bool DROP, bool SPLIT>
 __global__ void __launch_bounds__(BwdCfg<DKV, D>::kThreads, BwdCfg<DKV, D>::kCtasPerSM)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant__ CUtensorMap tm_a2,
                 const __grid_constant__ CUtensorMap tm_b1, const __grid_constant__ CUtensorMap tm_b2, const BwdParams p) {
@@ -190,18 +198,25 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
   uint64_t* done = ds_full + 1;         // the sums are complete
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
   int* s_count = reinterpret_cast<int*>(tmem_holder + 1);
+  int* s_last = s_count + 1;            // this CTA finishes the tile
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rows = DKV ? p.Ns : p.Nt;                  // of the resident side
   const int heads = DKV ? p.kv_heads : p.heads;
   const int tiles = (rows + kTileM - 1) / kTileM;
-  int head, tile;
+  int head, tile;                                      // and the CTA's part of the tile
   if (!p.by_head) {  // the first tiles of all heads first: with global tokens they are the longest
     tile = blockIdx.x / heads;
     head = blockIdx.x - tile * heads;
   } else {
-    head = blockIdx.x / tiles;
-    tile = blockIdx.x - head * tiles;
+    const int per_head = SPLIT ? tiles * p.split : tiles;
+    head = blockIdx.x / per_head;
+    tile = blockIdx.x - head * per_head;
+  }
+  int part = 0;
+  if constexpr (SPLIT) {
+    part = tile % p.split;
+    tile /= p.split;
   }
   const int blk0 = tile * 2;                           // first of the tile's two blocks
   const int nbr = p.Nt / kBlk, nbc = p.Ns / kBlk;
@@ -264,7 +279,22 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
   const int count = __shfl_sync(0xffffffffu, *s_count, 0);
   const int pairs = (count + C::kBlocks - 1) / C::kBlocks;  // steps through the list
-  const int steps = DKV ? pairs * p.group : pairs;     // dK, dV: the list once for every head that shares the keys
+  const int all_steps = DKV ? pairs * p.group : pairs;  // dK, dV: the list once for every head that shares the keys
+  // A tile whose steps would take one CTA far longer than the others (global tokens, heads that share their keys), or
+  // that is one of few, is shared by several CTAs, each with a range of the steps.  They leave 32-bit partial sums; the
+  // last one to finish adds them in their order.
+  int parts = 1, step0 = 0, steps = all_steps, h0 = 0, k0 = 0;  // step = h * pairs + k
+  if constexpr (SPLIT) {
+    parts = min(p.split, max(1, (all_steps + p.split_steps / 2) / p.split_steps));
+    if (part >= parts) {
+      if (warp == kWarpMma) tmem_dealloc<C::kTmemCols>(tmem_base);
+      return;
+    }
+    step0 = static_cast<int>((long long)all_steps * part / parts);
+    steps = static_cast<int>((long long)all_steps * (part + 1) / parts) - step0;
+    h0 = pairs > 0 ? step0 / pairs : 0;
+    k0 = step0 - h0 * pairs;
+  }
   const long long a_row0 = (long long)head * rows + (long long)tile * kTileM;
 
   bool failed = false;  // a bounded wait of this thread gave up
@@ -277,7 +307,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
         tma_load_2d(a2_s + c * (kTileM * 128), &tm_a2, c * 64, (int)a_row0, a_full);
       }
       bool ok = true;
-      int h = 0, k = 0;  // step = h * pairs + k
+      int h = h0, k = k0;
       for (int j = 0; j < steps; ++j) {
         const int st = j % kStages, nblk = min(C::kBlocks, count - C::kBlocks * k);
         const uint32_t par = ((j / kStages) & 1) ^ 1;
@@ -335,7 +365,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
                        (!first || kk > 0) ? 1u : 0u);
     };
     // the last pair of the list may be a single block
-    auto blocks_of = [&](int j) { return C::kBlocks == 2 && !((count & 1) && (j + 1) % pairs == 0) ? 2 : 1; };
+    auto blocks_of = [&](int j) { return C::kBlocks == 2 && !((count & 1) && (step0 + j + 1) % pairs == 0) ? 2 : 1; };
     bool ok = steps == 0 || mbar_wait_warp(a_full, 0);
 #pragma unroll
     for (int j = 0; j < kSBuf; ++j) {  // the first scores
@@ -441,7 +471,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
     const float up = p.drop.scale;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
-    int h = 0, k = 0;  // step = h * pairs + k
+    int h = h0, k = k0;
     for (int j = 0; j < steps; ++j) {
       const int st = j % kStages, at = C::kBlocks * k + (quarter >> 1);
       const int e = __shfl_sync(0xffffffffu, at < count ? ulist[at] : 0, 0);
@@ -558,32 +588,74 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
     }
-    // ---- epilogue: the sums -> global, one row per thread ----
+    // ---- epilogue: the sums -> global, one row per thread, 32-column pieces dealt to the threads of a row ----
     if (ok && steps > 0 && !mbar_wait_warp(done, 0)) ok = false;
     failed |= !ok;
     if (!ok && lane == 0) atomicExch(&p.status[3], 1);
     tc_fence_after_sync();
-    constexpr int kPieces = (DKV ? 2 : 1) * D / 32;    // 32-column pieces, dealt to the four threads of a row
-    for (int piece = quarter; piece < kPieces; piece += kScoreWarps / 4) {
-      const bool second = piece >= D / 32;             // dV
-      const int col = (piece - (second ? D / 32 : 0)) * 32;
-      uint32_t r[32];
+    constexpr int kPieces = (DKV ? 2 : 1) * D / 32;
+    const long long tile_id = (long long)head * tiles + tile;
+    // partial sums: [piece][float4 of the piece][row], so that a warp's accesses are contiguous
+    auto partial_at = [&](int of, int piece) {
+      return reinterpret_cast<float4*>(p.partial) + ((tile_id * p.split + of) * kPieces + piece) * (8 * kTileM) + row;
+    };
+    auto load_piece = [&](int piece, float (&v)[32]) {
       if (steps > 0 && ok) {
+        uint32_t r[32];
         tmem_ld_x32(tmem_base + lane_base + C::kAcc1 + piece * 32, r);
         tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) r[i] = 0;
+        for (int i = 0; i < 32; ++i) v[i] = 0.f;
       }
+    };
+    auto store_piece = [&](int piece, const float (&v)[32]) {
+      const bool second = piece >= D / 32;             // dV
       const float f = second ? (DROP ? up : 1.f) : p.scale;
-      uint32_t packed[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) packed[i] = pack2<T>(__uint_as_float(r[2 * i]) * f, __uint_as_float(r[2 * i + 1]) * f);
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(second ? p.out2 : p.out1) + (a_row0 + row) * D + (piece % (D / 32)) * 32);
       if (inside) {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(second ? p.out2 : p.out1) + (a_row0 + row) * D + col);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          dst[q] = make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+          dst[q] = make_uint4(pack2<T>(v[8 * q] * f, v[8 * q + 1] * f), pack2<T>(v[8 * q + 2] * f, v[8 * q + 3] * f),
+                              pack2<T>(v[8 * q + 4] * f, v[8 * q + 5] * f), pack2<T>(v[8 * q + 6] * f, v[8 * q + 7] * f));
+      }
+    };
+    if (!SPLIT || parts == 1) {
+      for (int piece = quarter; piece < kPieces; piece += kScoreWarps / 4) {
+        float v[32];
+        load_piece(piece, v);
+        store_piece(piece, v);
+      }
+    } else {
+      for (int piece = quarter; piece < kPieces; piece += kScoreWarps / 4) {
+        float v[32];
+        load_piece(piece, v);
+        float4* dst = partial_at(part, piece);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) __stcg(dst + q * kTileM, make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+      }
+      __threadfence();
+      named_barrier_sync(1, kScoreWarps * 32);
+      if (threadIdx.x == 0) *s_last = atomicAdd(p.tickets + tile_id, 1u) == static_cast<uint32_t>(parts - 1);
+      named_barrier_sync(1, kScoreWarps * 32);
+      if (*s_last) {  // the others' sums are in L2
+        __threadfence();
+        for (int piece = quarter; piece < kPieces; piece += kScoreWarps / 4) {
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          for (int of = 0; of < parts; ++of) {
+            const float4* src = partial_at(of, piece);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const float4 x = __ldcg(src + q * kTileM);
+              v[4 * q] += x.x; v[4 * q + 1] += x.y; v[4 * q + 2] += x.z; v[4 * q + 3] += x.w;
+            }
+          }
+          store_piece(piece, v);
+        }
       }
     }
   }
@@ -601,85 +673,150 @@ int rows_map(CUtensorMap* map, const void* base, int dtype, int D, long long row
   return make_tensor_map(map, base, dtype, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <bool DKV, int D, int FMT, bool MASK, bool DROP>
-int launch_pass(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2, const BwdParams& p,
-                cudaStream_t st) {
+// Tiles, CTAs per tile and steps per CTA of a pass.  Splitting aims at CTAs of half of what a resident CTA would have to
+// do if the work were dealt out evenly; `nnz` (kept blocks, 0 when unknown: no splitting) says how much there is, 0.65 of
+// it being what merging two block rows typically leaves.  A CTA takes kMinSteps steps at least: below that its fixed
+// costs and its partial sums (written once, read once) outweigh the balance.
+struct PassPlan {
+  int tiles, split, split_steps;
+  size_t partial_bytes;
+};
+constexpr int kMinSteps = 12, kMaxSplit = 16;
+constexpr size_t kMaxPartialBytes = size_t(256) << 20;
+
+template <bool DKV, int D>
+PassPlan plan_pass(int heads, int kv_heads, int Nt, int Ns, long long nnz) {
   using C = BwdCfg<DKV, D>;
-  auto kern = attn_bwd_kernel<DKV, D, FMT, MASK, DROP>;
+  const int h = DKV ? kv_heads : heads, rows = DKV ? Ns : Nt, stream = DKV ? Nt : Ns;
+  PassPlan plan;
+  plan.tiles = (rows + kTileM - 1) / kTileM;
+  const long long ctas = (long long)h * plan.tiles;
+  const long long most = (long long)((stream / kBlk + C::kBlocks - 1) / C::kBlocks) * (DKV ? heads / kv_heads : 1);  // steps of a tile
+  const double even = 0.65 * static_cast<double>(nnz) * heads / C::kBlocks / (kNumSMs * C::kCtasPerSM);
+  long long steps = static_cast<long long>(even / 2) + 1;
+  if (steps < kMinSteps) steps = kMinSteps;
+  const size_t bytes = sizeof(float) * kTileM * D * (DKV ? 2 : 1);
+  long long split = nnz > 0 ? (most + steps / 2) / steps : 1;
+  if (split > kMaxSplit) split = kMaxSplit;
+  while (split > 1 && ctas * split * bytes > kMaxPartialBytes) --split;
+  plan.split = split < 1 ? 1 : static_cast<int>(split);
+  if (plan.split == kMaxSplit) steps = (most + plan.split - 1) / plan.split > steps ? (most + plan.split - 1) / plan.split : steps;
+  plan.split_steps = static_cast<int>(steps > 0x3fffffff ? 0x3fffffff : steps);
+  plan.partial_bytes = plan.split > 1 ? ctas * plan.split * bytes : 0;
+  return plan;
+}
+
+template <bool DKV, int D, int FMT, bool MASK, bool DROP, bool SPLIT>
+int launch_pass(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2, BwdParams p,
+                const PassPlan& plan, cudaStream_t st) {
+  using C = BwdCfg<DKV, D>;
+  auto kern = attn_bwd_kernel<DKV, D, FMT, MASK, DROP, SPLIT>;
   static SmemAttrOnce attr;
   if (cudaError_t e = attr.ensure(kern, C::kSmem); e != cudaSuccess) return static_cast<int>(e);
-  const int rows = DKV ? p.Ns : p.Nt, heads = DKV ? p.kv_heads : p.heads;
-  const long long ctas = (long long)heads * ((rows + kTileM - 1) / kTileM);
+  const long long ctas = (long long)(DKV ? p.kv_heads : p.heads) * plan.tiles * plan.split;
+  if (ctas > 0x7fffffffll) return SPARTA_ERR_SHAPE;
+  p.split = plan.split;
+  p.split_steps = plan.split_steps;
   kern<<<static_cast<unsigned>(ctas), C::kThreads, C::kSmem, st>>>(a1, a2, b1, b2, p);
   return launch_status();
 }
 
+int present_pitch(int Ns) { return (Ns / kBlk + 1) & ~1; }
+size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
+
+struct Workspace {
+  size_t neg_lse, neg_delta, present, tickets_q, tickets_kv, partial, total;
+  long long n_tickets;
+  PassPlan q, kv;
+};
+template <int D>
+Workspace lay_out(int heads, int kv_heads, int Nt, int Ns, long long nnz) {
+  Workspace w;
+  w.q = plan_pass<false, D>(heads, kv_heads, Nt, Ns, nnz);
+  w.kv = plan_pass<true, D>(heads, kv_heads, Nt, Ns, nnz);
+  w.n_tickets = (long long)heads * w.q.tiles + (long long)kv_heads * w.kv.tiles;
+  w.neg_lse = 0;
+  w.neg_delta = w.neg_lse + round16(sizeof(float) * (size_t)heads * Nt);
+  w.present = w.neg_delta + round16(sizeof(float) * (size_t)heads * Nt);
+  w.tickets_q = w.present + round16((size_t)(Nt / kBlk) * present_pitch(Ns));
+  w.tickets_kv = w.tickets_q + sizeof(uint32_t) * (size_t)heads * w.q.tiles;
+  w.partial = w.tickets_q + round16(sizeof(uint32_t) * (size_t)w.n_tickets);
+  w.total = w.partial + (w.q.partial_bytes > w.kv.partial_bytes ? w.q.partial_bytes : w.kv.partial_bytes);  // one pass at a time
+  return w;
+}
+
 template <int D, int FMT, bool MASK, bool DROP>
-int launch_bwd(const AttnArgs& a, BwdParams p, float* neg_lse, float* neg_delta, uint8_t* present, cudaStream_t st) {
+int launch_bwd(const AttnArgs& a, BwdParams p, cudaStream_t st) {
   using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
+  const Workspace w = lay_out<D>(a.heads, a.kv_heads, a.Nt, a.Ns, a.nnz);
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  float* neg_lse = reinterpret_cast<float*>(ws + w.neg_lse);
+  float* neg_delta = reinterpret_cast<float*>(ws + w.neg_delta);
+  uint32_t* tickets_q = reinterpret_cast<uint32_t*>(ws + w.tickets_q);
+  p.neg_lse = neg_lse; p.neg_delta = neg_delta; p.present = ws + w.present;
+  p.partial = reinterpret_cast<float*>(ws + w.partial);
+  p.present_pitch = present_pitch(a.Ns);
   const long long q_rows = (long long)a.heads * a.Nt, k_rows = (long long)a.kv_heads * a.Ns;
   const long long ctas = (q_rows + 2048 / D - 1) / (2048 / D);
   attn_bwd_prep_kernel<T, D><<<static_cast<unsigned>(ctas), 256, 0, st>>>(
-      static_cast<const T*>(a.O), static_cast<const T*>(a.dO), a.lse, neg_lse, neg_delta, present, a.row_ptr, a.idx, q_rows,
-      a.Nt / kBlk, a.Ns / kBlk, p.present_pitch);
+      static_cast<const T*>(a.O), static_cast<const T*>(a.dO), a.lse, neg_lse, neg_delta, ws + w.present, a.row_ptr, a.idx, q_rows,
+      a.Nt / kBlk, a.Ns / kBlk, p.present_pitch, tickets_q, w.n_tickets);
   if (int rc = launch_status(); rc != SPARTA_OK) return rc;
-  CUtensorMap q128, do128, k64, v64, k128, v128, q64, do64;
-  int rc = rows_map(&q128, a.Q, a.dtype, D, q_rows, kTileM);
-  if (rc == SPARTA_OK) rc = rows_map(&do128, a.dO, a.dtype, D, q_rows, kTileM);
-  if (rc == SPARTA_OK) rc = rows_map(&k64, a.K, a.dtype, D, k_rows, kBlk);
-  if (rc == SPARTA_OK) rc = rows_map(&v64, a.V, a.dtype, D, k_rows, kBlk);
-  if (rc == SPARTA_OK) rc = rows_map(&k128, a.K, a.dtype, D, k_rows, kTileM);
-  if (rc == SPARTA_OK) rc = rows_map(&v128, a.V, a.dtype, D, k_rows, kTileM);
-  if (rc == SPARTA_OK) rc = rows_map(&q64, a.Q, a.dtype, D, q_rows, kBlk);
-  if (rc == SPARTA_OK) rc = rows_map(&do64, a.dO, a.dtype, D, q_rows, kBlk);
-  if (rc != SPARTA_OK) return rc;
-  p.out1 = a.dK; p.out2 = a.dV;
-  p.by_head = kv_exceeds_l2(a.heads, a.Nt, D);
-  if (a.dK) rc = launch_pass<true, D, FMT, MASK, DROP>(k128, v128, q64, do64, p, st);
-  if (rc != SPARTA_OK || !a.dQ) return rc;
-  p.out1 = a.dQ; p.out2 = nullptr;
-  p.by_head = kv_exceeds_l2(a.kv_heads, a.Ns, D);
-  return launch_pass<false, D, FMT, MASK, DROP>(q128, do128, k64, v64, p, st);
+  CUtensorMap a1, a2, b1, b2;
+  if (a.dK) {
+    int rc = rows_map(&a1, a.K, a.dtype, D, k_rows, kTileM);
+    if (rc == SPARTA_OK) rc = rows_map(&a2, a.V, a.dtype, D, k_rows, kTileM);
+    if (rc == SPARTA_OK) rc = rows_map(&b1, a.Q, a.dtype, D, q_rows, kBlk);
+    if (rc == SPARTA_OK) rc = rows_map(&b2, a.dO, a.dtype, D, q_rows, kBlk);
+    if (rc != SPARTA_OK) return rc;
+    p.out1 = a.dK; p.out2 = a.dV;
+    p.by_head = kv_exceeds_l2(a.heads, a.Nt, D);
+    p.tickets = reinterpret_cast<uint32_t*>(ws + w.tickets_kv);
+    rc = w.kv.split > 1 ? launch_pass<true, D, FMT, MASK, DROP, true>(a1, a2, b1, b2, p, w.kv, st)
+                        : launch_pass<true, D, FMT, MASK, DROP, false>(a1, a2, b1, b2, p, w.kv, st);
+    if (rc != SPARTA_OK) return rc;
+  }
+  if (a.dQ) {
+    int rc = rows_map(&a1, a.Q, a.dtype, D, q_rows, kTileM);
+    if (rc == SPARTA_OK) rc = rows_map(&a2, a.dO, a.dtype, D, q_rows, kTileM);
+    if (rc == SPARTA_OK) rc = rows_map(&b1, a.K, a.dtype, D, k_rows, kBlk);
+    if (rc == SPARTA_OK) rc = rows_map(&b2, a.V, a.dtype, D, k_rows, kBlk);
+    if (rc != SPARTA_OK) return rc;
+    p.out1 = a.dQ; p.out2 = nullptr;
+    p.by_head = kv_exceeds_l2(a.kv_heads, a.Ns, D);
+    p.tickets = tickets_q;
+    rc = w.q.split > 1 ? launch_pass<false, D, FMT, MASK, DROP, true>(a1, a2, b1, b2, p, w.q, st)
+                       : launch_pass<false, D, FMT, MASK, DROP, false>(a1, a2, b1, b2, p, w.q, st);
+    if (rc != SPARTA_OK) return rc;
+  }
+  return SPARTA_OK;
 }
 
 template <int D, int FMT>
-int launch_variant(const AttnArgs& a, const BwdParams& p, float* neg_lse, float* neg_delta, uint8_t* present, cudaStream_t st) {
+int launch_variant(const AttnArgs& a, const BwdParams& p, cudaStream_t st) {
   const bool drop = p.drop.threshold > 0;
-  if (a.mask) return drop ? launch_bwd<D, FMT, true, true>(a, p, neg_lse, neg_delta, present, st)
-                          : launch_bwd<D, FMT, true, false>(a, p, neg_lse, neg_delta, present, st);
-  return drop ? launch_bwd<D, FMT, false, true>(a, p, neg_lse, neg_delta, present, st)
-              : launch_bwd<D, FMT, false, false>(a, p, neg_lse, neg_delta, present, st);
+  if (a.mask) return drop ? launch_bwd<D, FMT, true, true>(a, p, st)
+                          : launch_bwd<D, FMT, true, false>(a, p, st);
+  return drop ? launch_bwd<D, FMT, false, true>(a, p, st)
+              : launch_bwd<D, FMT, false, false>(a, p, st);
 }
-
-int present_pitch(int Ns) { return (Ns / kBlk + 1) & ~1; }
-size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
-size_t stat_bytes(int heads, int Nt) { return round16(sizeof(float) * (size_t)heads * Nt); }
 
 }  // namespace
 
-size_t attn_bwd_workspace(int heads, int Nt, int Ns) {
-  return 2 * stat_bytes(heads, Nt) + round16((size_t)(Nt / kBlk) * present_pitch(Ns));
+size_t attn_bwd_workspace(int heads, int kv_heads, int Nt, int Ns, int D, long long nnz) {
+  return D == 64 ? lay_out<64>(heads, kv_heads, Nt, Ns, nnz).total : lay_out<128>(heads, kv_heads, Nt, Ns, nnz).total;
 }
 
 int attn_bwd_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* status, cudaStream_t st) {
   if (a.Ns / kBlk > kMaxBlocks || a.Nt / kBlk > kMaxBlocks) return SPARTA_ERR_UNSUPPORTED;
   BwdParams p = {};
-  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-  float* neg_lse = reinterpret_cast<float*>(ws);
-  float* neg_delta = reinterpret_cast<float*>(ws + stat_bytes(a.heads, a.Nt));
-  uint8_t* present = ws + 2 * stat_bytes(a.heads, a.Nt);
-  p.row_ptr = a.row_ptr; p.idx = a.idx; p.mask = a.mask; p.present = present;
-  p.neg_lse = neg_lse; p.neg_delta = neg_delta;
+  p.row_ptr = a.row_ptr; p.idx = a.idx; p.mask = a.mask;
   p.Nt = a.Nt; p.Ns = a.Ns; p.heads = a.heads; p.kv_heads = a.kv_heads; p.group = a.heads / a.kv_heads;
-  p.present_pitch = present_pitch(a.Ns);
   p.scale = a.scale; p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = status;
   p.drop = drop;
-  if (a.D == 64)
-    return a.dtype == SPARTA_F16 ? launch_variant<64, 0>(a, p, neg_lse, neg_delta, present, st)
-                                 : launch_variant<64, 1>(a, p, neg_lse, neg_delta, present, st);
-  return a.dtype == SPARTA_F16 ? launch_variant<128, 0>(a, p, neg_lse, neg_delta, present, st)
-                               : launch_variant<128, 1>(a, p, neg_lse, neg_delta, present, st);
+  if (a.D == 64) return a.dtype == SPARTA_F16 ? launch_variant<64, 0>(a, p, st) : launch_variant<64, 1>(a, p, st);
+  return a.dtype == SPARTA_F16 ? launch_variant<128, 0>(a, p, st) : launch_variant<128, 1>(a, p, st);
 }
 
 }  // namespace sparta

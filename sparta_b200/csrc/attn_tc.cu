@@ -557,6 +557,8 @@ int train_args(const sparta_attn_train_args* h, AttnArgs* a, DropoutParams* drop
   a->kv_heads = h->kv_heads;
   a->dO = h->dO; a->dQ = h->dQ; a->dK = h->dK; a->dV = h->dV;
   a->workspace = h->workspace;
+  a->nnz = h->nnz_hint;
+  if (h->nnz_hint < 0) return SPARTA_ERR_BAD_ARG;
   if (!aligned(h->lse, 4) || (h->rng && !aligned(h->rng, 8))) return SPARTA_ERR_ALIGN;
   if (!make_dropout(drop, h->dropout, h->rng, h->seed, h->call)) return SPARTA_ERR_BAD_ARG;
   return check_attn(*a, h->BLK);
@@ -598,9 +600,9 @@ extern "C" int sparta_attn_train_fwd(const sparta_attn_train_args* h_args, void*
   return attn_fwd_entry(a, h_args->BLK, drop, h_args->status, nullptr, 0, stream);
 }
 
-extern "C" size_t sparta_attn_train_bwd_workspace_bytes(int heads, int Nt, int Ns) {
-  if (heads <= 0 || Nt <= 0 || Ns <= 0) return 0;
-  return attn_bwd_workspace(heads, Nt, Ns);
+extern "C" size_t sparta_attn_train_bwd_workspace_bytes(int heads, int kv_heads, int Nt, int Ns, int D, int64_t nnz_hint) {
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || Nt <= 0 || Ns <= 0 || (D != 64 && D != 128) || nnz_hint < 0) return 0;
+  return attn_bwd_workspace(heads, kv_heads, Nt, Ns, D, nnz_hint);
 }
 
 extern "C" int sparta_attn_train_bwd(const sparta_attn_train_args* h_args, void* stream) {
@@ -609,7 +611,7 @@ extern "C" int sparta_attn_train_bwd(const sparta_attn_train_args* h_args, void*
   if (int rc = train_args(h_args, &a, &drop); rc != SPARTA_OK) return rc;
   if (!a.lse || !a.dO || !a.dK != !a.dV || (!a.dQ && !a.dK)) return SPARTA_ERR_BAD_ARG;
   if (!aligned(a.dO, 16) || !aligned(a.dQ, 16) || !aligned(a.dK, 16) || !aligned(a.dV, 16)) return SPARTA_ERR_ALIGN;
-  if (!a.workspace || h_args->workspace_bytes < attn_bwd_workspace(a.heads, a.Nt, a.Ns)) return SPARTA_ERR_WORKSPACE;
+  if (!a.workspace || h_args->workspace_bytes < attn_bwd_workspace(a.heads, a.kv_heads, a.Nt, a.Ns, a.D, a.nnz)) return SPARTA_ERR_WORKSPACE;
   if (!aligned(a.workspace, 16)) return SPARTA_ERR_ALIGN;
   int32_t* status = h_args->status ? h_args->status : tc::device_status_ptr();
   if (!status) return SPARTA_ERR_DRIVER;

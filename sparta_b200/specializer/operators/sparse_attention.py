@@ -166,7 +166,7 @@ class SparseAttention(OperatorBase):
         return _lib.AttnTrainArgs(  # in the order of its fields
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), None, None, None, None, None, 0,
             indexes.row_ptr.data_ptr(), indexes.bcsr_buf.data_ptr(), _lib.ptr(mask), _lib.ptr(numbers.rng),
-            numbers.seed & 0xffffffffffffffff, numbers.call & 0xffffffff, self._attn_status.data_ptr(), p, self._scale,
+            numbers.seed & 0xffffffffffffffff, numbers.call & 0xffffffff, indexes.block_nnz, self._attn_status.data_ptr(), p, self._scale,
             q.shape[0], k.shape[0], self._Nt, self._Ns, q.shape[2], FUSED_BLOCK, _lib.dtype_code(q))
 
     def _raise_on_status(self):
@@ -194,8 +194,8 @@ class SparseAttention(OperatorBase):
         if not (want_q or want_kv):
             return dq, dk, dv
         L = _lib.lib()
-        ws = torch.empty(L.sparta_attn_train_bwd_workspace_bytes(q.shape[0], self._Nt, self._Ns), dtype=torch.uint8,
-                         device=q.device)
+        ws = torch.empty(L.sparta_attn_train_bwd_workspace_bytes(q.shape[0], k.shape[0], self._Nt, self._Ns, q.shape[2],
+                                                                 indexes.block_nnz), dtype=torch.uint8, device=q.device)
         args = self._train_args(q, k, v, out, lse, indexes, mask, p, numbers)
         args.dO, args.dQ, args.dK, args.dV = grad.data_ptr(), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv)
         args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()

@@ -15,7 +15,7 @@ def args(**kw):
 
 
 def test_struct_layout():
-    assert ctypes.sizeof(_lib.AttnTrainArgs) == 15 * 8 + 2 * 8 + 8 + 8 + 8 * 4
+    assert ctypes.sizeof(_lib.AttnTrainArgs) == 15 * 8 + 3 * 8 + 8 + 8 + 8 * 4
     assert ctypes.sizeof(_lib.RotaryTensor) == 3 * 8 + 3 * 8 + 4 * 4
 
 
@@ -41,8 +41,15 @@ def test_refusals():
         assert bwd(args(**kw), None) == -1
     for name in ('dO', 'dQ', 'dK', 'dV', 'workspace'):
         assert bwd(args(**{name: FAKE + 8}), None) == -5
-    need = L.sparta_attn_train_bwd_workspace_bytes(4, 128, 192)
+    need = L.sparta_attn_train_bwd_workspace_bytes(4, 2, 128, 192, 64, 0)
     assert need >= 2 * 4 * 128 * 4 + 2 * 3
     assert bwd(args(workspace_bytes=need - 1), None) == -4 and bwd(args(workspace=None), None) == -4
     assert bwd(args(Nt=65536 + 64), None) == -3
-    assert L.sparta_attn_train_bwd_workspace_bytes(0, 128, 128) == 0
+    assert bwd(args(nnz_hint=-1), None) == -1
+    for bad in ((0, 1, 128, 128, 64, 0), (4, 3, 128, 128, 64, 0), (4, 2, 128, 128, 96, 0), (4, 2, 128, 128, 64, -1)):
+        assert L.sparta_attn_train_bwd_workspace_bytes(*bad) == 0
+    # tiles that several CTAs share leave partial sums in the workspace: it grows with the kept blocks up to a bound
+    long = (4, 1, 65536, 65536, 128)
+    sizes = [L.sparta_attn_train_bwd_workspace_bytes(*long, n) for n in (0, 2000, 20000, 1 << 20)]
+    assert sizes[0] < sizes[1] and sizes[0] == sizes[3] and max(sizes) <= sizes[0] + (256 << 20)
+    assert bwd(args(workspace_bytes=need, nnz_hint=0, workspace=None), None) == -4

@@ -101,7 +101,9 @@ def step(op, q, k, v, do, **kw):
 SHAPES = [  # heads, kv_heads, nt, ns, share of blocks, element mask
     (1, 1, 64, 64, 1.0, False), (2, 2, 128, 128, 1.0, False), (3, 3, 64, 192, 1.0, False), (2, 2, 320, 64, 0.7, False),
     (2, 1, 256, 448, 0.5, False), (6, 2, 192, 320, 0.5, True), (4, 4, 512, 512, 0.3, False), (1, 1, 128, 1088, 0.6, True),
-    (8, 2, 576, 256, 0.4, False), (2, 2, 256, 256, 0.4, True)]
+    (8, 2, 576, 256, 0.4, False), (2, 2, 256, 256, 0.4, True),
+    # few tiles with many steps: several CTAs share a tile and add their partial sums
+    (1, 1, 2048, 192, 0.8, False), (4, 1, 1088, 128, 0.9, True), (2, 2, 64, 4096, 0.7, False), (1, 1, 4160, 4032, 0.5, False)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
