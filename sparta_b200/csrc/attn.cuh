@@ -69,62 +69,8 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float v0, float v1) {
 __device__ __forceinline__ uint32_t to_split32(uint32_t c) { return (c >> 1) | ((c & 1u) << 4); }        // column -> bit
 __device__ __forceinline__ uint32_t from_split32(uint32_t i) { return ((i & 15u) << 1) | (i >> 4); }  // bit -> column
 
-// ---- the generator for a row of the score matrix ----
-// The counter is (column / 8, row, batch element, call).  After two of the seven rounds two of the four words depend on
-// (column, batch element) alone and two on the row as well, so that of fourteen products nine are left that depend on
-// both; a row's own product is made once, and those of the column are the same for a whole warp.
-struct PhiloxRow {
-  uint32_t hi, lo;  // of the second round's product, the key in `hi`
-};
-__device__ __forceinline__ PhiloxRow philox_row(const PhiloxKey& key, uint32_t row, uint32_t batch) {
-  const uint32_t x0 = __umulhi(0xCD9E8D57u, batch) ^ row ^ key.k0;
-  const uint64_t a = static_cast<uint64_t>(0xD2511F53u) * x0;
-  return {static_cast<uint32_t>(a >> 32) ^ (key.k1 + 0xBB67AE85u), static_cast<uint32_t>(a)};
-}
-__device__ __forceinline__ void philox8_row(const PhiloxKey& key, const PhiloxRow& r, uint32_t g, uint32_t batch, uint32_t (&w)[4]) {
-  constexpr uint32_t kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u, kW0 = 0x9E3779B9u, kW1 = 0xBB67AE85u;
-  const uint64_t a1 = static_cast<uint64_t>(kM0) * g;
-  const uint64_t b2 = static_cast<uint64_t>(kM1) * (static_cast<uint32_t>(a1 >> 32) ^ key.call ^ key.k1);
-  const uint64_t a3 = static_cast<uint64_t>(kM0) * (static_cast<uint32_t>(b2 >> 32) ^ (kM1 * batch) ^ (key.k0 + kW0));
-  const uint64_t b3 = static_cast<uint64_t>(kM1) * (r.hi ^ static_cast<uint32_t>(a1));
-  uint32_t x0 = static_cast<uint32_t>(b3 >> 32) ^ (static_cast<uint32_t>(b2) ^ (key.k0 + 2 * kW0));
-  uint32_t x1 = static_cast<uint32_t>(b3);
-  uint32_t x2 = (static_cast<uint32_t>(a3 >> 32) ^ (key.k1 + 2 * kW1)) ^ r.lo;
-  uint32_t x3 = static_cast<uint32_t>(a3);
-#pragma unroll
-  for (int i = 3; i < 7; ++i) {
-    const uint64_t a = static_cast<uint64_t>(kM0) * x0, b = static_cast<uint64_t>(kM1) * x2;
-    x0 = static_cast<uint32_t>(b >> 32) ^ x1 ^ (key.k0 + i * kW0);
-    x1 = static_cast<uint32_t>(b);
-    x2 = static_cast<uint32_t>(a >> 32) ^ x3 ^ (key.k1 + i * kW1);
-    x3 = static_cast<uint32_t>(a);
-  }
-  w[0] = x0; w[1] = x1; w[2] = x2; w[3] = x3;
-}
-// the same key in every lane, known to the compiler as such
-__device__ __forceinline__ PhiloxKey load_uniform_philox_key(const DropoutParams& d) {
-  const PhiloxKey k = load_philox_key(d);
-  return {__shfl_sync(0xffffffffu, k.k0, 0), __shfl_sync(0xffffffffu, k.k1, 0), __shfl_sync(0xffffffffu, k.call, 0)};
-}
-
-// Bits 15 and 31: the halves of w are not below the halves of t (a threshold below 65536 twice).  Side by side: with
-// the top bits set aside, a subtraction of the lower 15 bits leaves its borrow in place of the top bit, and the result
-// is decided by the top bits or, where they agree, by that.
-__device__ __forceinline__ uint32_t not_below2(uint32_t w, uint32_t t) {
-  const uint32_t d = (w | 0x80008000u) - (t & 0x7fff7fffu);
-  return (w & ~t) | (~(w ^ t) & d);
-}
-// bits 15 and 31 over their halves
-__device__ __forceinline__ uint32_t spread2(uint32_t x) {
-  uint32_t m;
-  asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(m) : "r"(x));  // sign of byte 1, byte 3 over two bytes each
-  return m;
-}
 // 0xffff in each half whose bit (i, 16 + i) is set
 __device__ __forceinline__ uint32_t pair_mask(uint32_t word, int i) { return spread2(word << (15 - i)); }
-
-// The threshold in both halves.  "Everything dropped" (65536) becomes "nothing": its scale is 0.
-__device__ __forceinline__ uint32_t threshold2(const DropoutParams& d) { return (d.threshold & 0xffffu) * 0x00010001u; }
 
 // 32 dropout decisions of columns 32 g .. of a row, split order
 __device__ __forceinline__ uint32_t philox_split32(const PhiloxKey& key, const PhiloxRow& r, uint32_t t2, uint32_t g, uint32_t batch) {
@@ -132,7 +78,7 @@ __device__ __forceinline__ uint32_t philox_split32(const PhiloxKey& key, const P
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint32_t w[4];
-    philox8_row(key, r, 4 * g + q, batch, w);
+    philox8(key, r, philox_col(key, 4 * g + q, batch), w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) bits = (bits >> 1) | (not_below2(w[i], t2) & 0x80008000u);
   }
@@ -143,7 +89,7 @@ __device__ __forceinline__ void drop_packed32(uint32_t* packed, const PhiloxKey&
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint32_t w[4];
-    philox8_row(key, r, 4 * g + q, batch, w);
+    philox8(key, r, philox_col(key, 4 * g + q, batch), w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) packed[4 * q + i] &= spread2(not_below2(w[i], t2));
   }

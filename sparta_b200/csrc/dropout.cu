@@ -1,22 +1,24 @@
 // Dropout whose decisions come from a counter and are never stored:  y = keep(b, r, c) ? x * scale : 0  (philox.cuh).
 // The backward pass is the same function of the output gradient, so one kernel serves both directions.
 //
-// Bound by HBM: one read and one write per element.  A Philox call (about 45 instructions for 8 decisions) and its
-// compares must stay below the ~20 instructions per 16-bit element that the SMs can issue while HBM moves it, so a
-// call is made once per group of eight columns:
-//   * a thread owns a 16-byte aligned piece of memory (8 elements, or two pieces for fp32) per step, four steps,
-//     all loads issued first;
-//   * rows whose length is a multiple of 8: the piece is one group, one call;
-//   * other rows: the piece straddles two groups.  Each lane makes the call of its piece's LAST group; the bits of
-//     the group before it are what the lane below (or lane 31 of the step before) has just made, and only the first
-//     step of a warp, and pieces that hold a row's end, call twice.
+// Bound by HBM: one read and one write per element, which leaves the SMs about 20 instructions per 16-bit element.  A
+// thread owns 16 bytes of 16-bit elements (32 of fp32), one call of the generator, at the same place of several rows:
+// the column's share of the generator is made once for all of them, the row's share once per row, and the decisions
+// are applied to packed pairs (with a full call and a compare and a select per element the kernel issued 23
+// instructions per element and took 119 us for 134 M bf16 elements; now see the table in the design notes).
+// Rows whose length is no multiple of 8 begin anywhere in a 16-byte piece of memory.  Pieces stay aligned, so that a
+// piece holds the end of one group of eight columns and the beginning of the next: each lane makes the decisions of the
+// group that begins in its piece and takes those of the group before from the lane below (the lowest lane of a segment
+// only makes them).  Pieces at either end of a row are handled element by element.
 #include "philox.cuh"
 
 namespace sparta {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSteps = 4;   // pieces per thread
+template <typename T>
+constexpr int kBatch = 8 / sizeof(T);  // rows whose loads are in flight together: 64 bytes per thread
+constexpr int kMaxRows = 8; // rows per thread, or 1 where rows are few
 constexpr int kPiece = 8;   // elements per piece = decisions per generator call
 
 template <typename T>
@@ -42,77 +44,120 @@ __device__ __forceinline__ void store_piece(T* p, const Piece<T>& r) {
 #pragma unroll
   for (int i = 0; i < n; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(r.v)[i];
 }
+// Scale a pair and keep what `mask` covers.  Masked bits, not a product with zero: NaN and infinities are dropped too.
+// The product is taken in 32 bits and rounded once.
 template <typename T>
-__device__ __forceinline__ T drop(T v, bool keep, float scale) {
-  return keep ? from_float<T>(to_float(v) * scale) : from_float<T>(0.f);  // a select: NaN and infinities are dropped too
+__device__ __forceinline__ void drop_pair(Piece<T>& p, int i, uint32_t mask, float scale) {
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t lo = __byte_perm(mask, 0, 0x1010), hi = __byte_perm(mask, 0, 0x3232);
+    p.v[2 * i] = __uint_as_float(__float_as_uint(p.v[2 * i] * scale) & lo);
+    p.v[2 * i + 1] = __uint_as_float(__float_as_uint(p.v[2 * i + 1] * scale) & hi);
+  } else {
+    const T a = from_float<T>(to_float(p.v[2 * i]) * scale), b = from_float<T>(to_float(p.v[2 * i + 1]) * scale);
+    T two[2] = {a, b};
+    reinterpret_cast<uint32_t*>(p.v)[i] = *reinterpret_cast<const uint32_t*>(two) & mask;
+  }
 }
 
-// Dense [batch, H, W]; y 16-byte aligned, VEC: x too.  EVEN: W % 8 == 0.
-template <typename T, bool EVEN, bool VEC>
-__global__ void __launch_bounds__(kThreads)
-dropout_dense_kernel(const T* __restrict__ x, T* __restrict__ y, long long n, int H, int W, DropoutParams d) {
-  const int lane = threadIdx.x & 31;
-  const long long warp0 = ((long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * (32 * kSteps * kPiece);
-  if (warp0 >= n) return;  // whole warps only: the shuffles below need every lane
-  const PhiloxKey key = load_philox_key(d);
-  const bool none = d.threshold >= kDropoutOne;
-  const uint32_t cut = d.threshold << 16;
-  // position of the warp's first element; a lane's position is that plus a 32-bit offset
-  const long long row0 = warp0 / W;
-  const uint32_t col0 = static_cast<uint32_t>(warp0 - row0 * W);
-  const long long b0 = row0 / H;
-  const uint32_t r0 = static_cast<uint32_t>(row0 - b0 * H);
-
-  Piece<T> in[kSteps];
+// The masks of a piece's four pairs.  Rows that are no multiple of 8 long begin `a` elements into a piece: the piece then
+// holds the last `a` columns of the group before the lane's own (whose decisions the lane below made) and the first
+// 8 - a of its own.  Every lane of the warp calls it.
+template <bool EVEN>
+__device__ __forceinline__ void piece_masks(const PhiloxKey& key, const PhiloxRow& row, const PhiloxCol& col, uint32_t t2, int a, int seg,
+                                            uint32_t (&mask)[4]) {
+  uint32_t w[4];
+  philox8(key, row, col, w);
+  if constexpr (EVEN) {
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const long long e = warp0 + (s * 32 + lane) * kPiece;
-    if (e + kPiece <= n) in[s] = load_piece<T, VEC>(x + e);
-    else if (e < n)
-      for (int i = 0; i < kPiece; ++i) in[s].v[i] = e + i < n ? x[e + i] : from_float<T>(0.f);
+    for (int i = 0; i < 4; ++i) mask[i] = spread2(not_below2(w[i], t2));
+  } else {
+    uint32_t own = 0;  // decisions of columns 2 i, 2 i + 1 at bits 2 i, 2 i + 16, then side by side
+#pragma unroll
+    for (int i = 0; i < 4; ++i) own |= (not_below2(w[i], t2) >> (15 - 2 * i)) & (0x00010001u << (2 * i));
+    own = (own | (own >> 15)) & 0xffu;
+    const uint32_t before = __shfl_up_sync(0xffffffffu, own, 1, seg);
+    uint32_t bits = (before | (own << 8)) >> (8 - a);
+    bits |= bits << 15;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mask[i] = spread2(bits << (15 - 2 * i));
   }
-  uint32_t carry = 0;  // bits of lane 31's last group in the step before
+}
+
+// Dense [rows, W], rows = batch * H; y 16-byte aligned, VEC: x too.  EVEN: W % 8 == 0.  A warp is 32 >> log_seg segments
+// of 1 << log_seg lanes, each on a row of its own; rows longer than a segment reaches are cut into `chunks`.
+template <typename T, bool EVEN, bool VEC>
+__global__ void __launch_bounds__(kThreads, 4)  // 64 registers: the loads of many warps hide each other
+dropout_dense_kernel(const T* __restrict__ x, T* __restrict__ y, long long rows, int H, int W, int log_seg, int chunks,
+                     int per_thread, DropoutParams d) {
+  const PhiloxKey key = load_uniform_philox_key(d);
+  const uint32_t t2 = threshold2(d);
+  const int lane = threadIdx.x & 31, seg = 1 << log_seg, at = lane & (seg - 1), per_warp = 32 >> log_seg;
+  const long long warp = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const long long group = warp / chunks;
+  const int chunk = static_cast<int>(warp - group * chunks);
+  const long long row0 = group * per_thread * per_warp;
+  if (row0 >= rows) return;  // whole warps only: the shuffles need every lane
+  // the group of columns whose decisions this lane makes, which begins in (or, EVEN, is) its piece of every row
+  const int m0 = EVEN ? chunk * seg : chunk * (seg - 1) - 1, m = m0 + at;
+  const bool makes_only = !EVEN && at == 0;
+  long long row = row0 + (lane >> log_seg);
+  uint32_t b = static_cast<uint32_t>(row / H), r = static_cast<uint32_t>(row - (long long)b * H);
+  PhiloxCol col = philox_col(key, m, b);
+  auto next_row = [&] {
+    r += per_warp;
+    if (r >= static_cast<uint32_t>(H)) {
+      b += r / H;
+      r %= H;
+      col = philox_col(key, m, b);
+    }
+  };
+  if (d.threshold < kDropoutOne && (EVEN || m0 >= 0) && m0 + seg <= W / kPiece && per_thread >= kBatch<T> &&
+      row0 + per_thread * per_warp <= rows) {
+    // ---- every piece of the warp is whole: loads of four rows in flight ----
+    const long long step = (long long)per_warp * W;
+    long long start = row * W;  // of the row, in elements
+#pragma unroll 1
+    for (int k0 = 0; k0 < per_thread; k0 += kBatch<T>) {
+      Piece<T> in[kBatch<T>];
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const long long e = warp0 + (s * 32 + lane) * kPiece;
-    const uint32_t off = col0 + (s * 32 + lane) * kPiece;
-    const uint32_t over = off / static_cast<uint32_t>(W);
-    uint32_t c = off - over * W;  // column, row and batch element of the piece's first element
-    uint32_t r = r0 + over, b = static_cast<uint32_t>(b0);
-    if (r >= static_cast<uint32_t>(H)) { b += r / H; r %= H; }
-    uint32_t bits;
-    if constexpr (EVEN) {
-      bits = philox_keep8(key, cut, c >> 3, r, b);
-    } else {
-      const uint32_t a = c & 7u;  // the piece begins at place a of group c / 8
-      const bool ends = c + kPiece > static_cast<uint32_t>(W);  // the row ends inside the piece
-      const uint32_t own = philox_keep8(key, cut, (c + kPiece - 1) >> 3, r, b);
-      uint32_t before = __shfl_up_sync(0xffffffffu, own, 1);
-      if (lane == 0) before = carry;
-      carry = __shfl_sync(0xffffffffu, own, 31);
-      // the lane below made the call of group c / 8 unless its piece reached over a row's end (then c < 8)
-      if (a != 0 && ((s == 0 && lane == 0) || c < 8)) before = philox_keep8(key, cut, c >> 3, r, b);
-      bits = a == 0 ? own : ((before | (own << 8)) >> a);
-      if (ends) {  // element by element across the row's end (rows shorter than a piece wrap several times)
-        bits = 0;
-        uint32_t grp = 0xffffffffu, g8 = 0;
-        for (int i = 0; i < kPiece; ++i) {
-          if ((c >> 3) != grp) { grp = c >> 3; g8 = philox_keep8(key, cut, grp, r, b); }
-          bits |= ((g8 >> (c & 7u)) & 1u) << i;
-          if (++c == static_cast<uint32_t>(W)) {
-            c = 0; grp = 0xffffffffu;
-            if (++r == static_cast<uint32_t>(H)) { r = 0; ++b; }
-          }
-        }
+      for (int k = 0; k < kBatch<T>; ++k)
+        if (!makes_only) in[k] = load_piece<T, VEC>(x + (((start + k * step) >> 3) + m) * kPiece);
+#pragma unroll
+      for (int k = 0; k < kBatch<T>; ++k) {
+        uint32_t mask[4];
+        piece_masks<EVEN>(key, philox_row(key, r, b), col, t2, static_cast<int>(start) & 7, seg, mask);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) drop_pair(in[k], i, mask[i], d.scale);
+        if (!makes_only) store_piece(y + ((start >> 3) + m) * kPiece, in[k]);
+        start += step;
+        next_row();
       }
     }
-    if (none) bits = 0;
+    return;
+  }
+  // ---- ends of rows, the last rows, and p = 1: piece by piece, whole or in part ----
+#pragma unroll 1
+  for (int k = 0; k < per_thread; ++k, row += per_warp) {
+    const long long start = row * W;
+    const int a = EVEN ? 0 : static_cast<int>(start & 7), c0 = kPiece * m - a;  // column of the piece's first element
+    uint32_t mask[4];
+    piece_masks<EVEN>(key, philox_row(key, r, b), col, t2, a, seg, mask);
+    if (d.threshold >= kDropoutOne) mask[0] = mask[1] = mask[2] = mask[3] = 0;
+    const int lo = max(0, -c0), hi = makes_only || row >= rows ? 0 : min(kPiece, W - c0);
+    if (lo == 0 && hi == kPiece) {
+      Piece<T> in = load_piece<T, VEC>(x + start + c0);
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) in[s].v[i] = drop(in[s].v[i], (bits >> i) & 1u, d.scale);
-    if (e + kPiece <= n) store_piece(y + e, in[s]);
-    else if (e < n)
+      for (int i = 0; i < 4; ++i) drop_pair(in, i, mask[i], d.scale);
+      store_piece(y + start + c0, in);
+    } else {
+#pragma unroll
       for (int i = 0; i < kPiece; ++i)
-        if (e + i < n) y[e + i] = in[s].v[i];
+        if (i >= lo && i < hi) {
+          const bool keep = (mask[i / 2] >> (16 * (i & 1))) & 1u;
+          y[start + c0 + i] = keep ? from_float<T>(to_float(x[start + c0 + i]) * d.scale) : from_float<T>(0.f);
+        }
+    }
+    next_row();
   }
 }
 
@@ -121,52 +166,62 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 dropout_blocks_kernel(const T* __restrict__ x, T* __restrict__ y, const int32_t* __restrict__ idx,
                       const int32_t* __restrict__ nnz, int log_bh, int log_bw, long long stride, long long pieces, DropoutParams d) {
-  const PhiloxKey key = load_philox_key(d);
+  const PhiloxKey key = load_uniform_philox_key(d);
+  const uint32_t t2 = threshold2(d);
   const bool none = d.threshold >= kDropoutOne;
-  const uint32_t cut = d.threshold << 16;
   const uint32_t batch = blockIdx.y;
   const int log_pb = log_bh + log_bw - 3;  // pieces per block
   const long long base = (long long)batch * (stride << (log_bh + log_bw));
   const int kept = __ldg(nnz);
-  Piece<T> in[kSteps];
-  const long long first = (long long)blockIdx.x * (kThreads * kSteps) + threadIdx.x;
+  Piece<T> in[kBatch<T>];
+  const long long first = (long long)blockIdx.x * (kThreads * kBatch<T>) + threadIdx.x;
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
+  for (int s = 0; s < kBatch<T>; ++s) {
     const long long v = first + s * kThreads;
     if (v < pieces) in[s] = load_piece<T, VEC>(x + base + v * kPiece);
   }
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
+  for (int s = 0; s < kBatch<T>; ++s) {
     const long long v = first + s * kThreads;
     if (v >= pieces) continue;
     const long long blk = v >> log_pb;
     const uint32_t in_blk = static_cast<uint32_t>(v - (blk << log_pb)) << 3;
-    uint32_t bits = 0;
-    if (blk < kept && !none) {  // values behind the last block of a mask come out as zeros
+    uint32_t w[4] = {0, 0, 0, 0};
+    const bool there = blk < kept && !none;  // values behind the last block of a mask come out as zeros
+    if (there) {
       const uint32_t entry = static_cast<uint32_t>(__ldg(idx + blk));
       const uint32_t row = ((entry >> 16) << log_bh) + (in_blk >> log_bw);
       const uint32_t col = ((entry & 0xffffu) << log_bw) + (in_blk & ((1u << log_bw) - 1u));
-      bits = philox_keep8(key, cut, col >> 3, row, batch);
+      philox8(key, philox_row(key, row, batch), philox_col(key, col >> 3, batch), w);
     }
 #pragma unroll
-    for (int i = 0; i < kPiece; ++i) in[s].v[i] = drop(in[s].v[i], (bits >> i) & 1u, d.scale);
+    for (int i = 0; i < 4; ++i) drop_pair(in[s], i, there ? spread2(not_below2(w[i], t2)) : 0u, d.scale);
     store_piece(y + base + v * kPiece, in[s]);
   }
 }
 
 template <typename T>
-int launch_dense(const void* x, void* y, long long n, int H, int W, const DropoutParams& d, cudaStream_t st) {
-  const long long per_cta = (long long)kThreads * kSteps * kPiece;
-  const long long ctas = (n + per_cta - 1) / per_cta;
+int launch_dense(const void* x, void* y, long long rows, int H, int W, const DropoutParams& d, cudaStream_t st) {
+  const bool even = W % kPiece == 0;
+  const int pieces = even ? W / kPiece : (W + 2 * kPiece - 2) / kPiece;  // of a row, wherever in a piece it begins
+  int log_seg = even ? 0 : 1;
+  while (log_seg < 5 && (1 << log_seg) - (even ? 0 : 1) < pieces) ++log_seg;
+  const int reach = (1 << log_seg) - (even ? 0 : 1), chunks = (pieces + reach - 1) / reach;
+  // several rows per thread share the column's part of the generator and have their loads in flight together; with fewer
+  // than 16 warps per SM it is the latency of one row that counts
+  const int per_thread = (rows >> (5 - log_seg)) * chunks / kMaxRows >= 16 * kNumSMs ? kMaxRows : 1;
+  const long long per_group = (long long)per_thread * (32 >> log_seg);
+  const long long warps = (rows + per_group - 1) / per_group * chunks;
+  const long long ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
   if (ctas > 0x7fffffffll) return SPARTA_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(ctas));
   const T* px = static_cast<const T*>(x);
   T* py = static_cast<T*>(y);
-  const bool vec = aligned(x, 16), even = W % 8 == 0;
-  if (even && vec) dropout_dense_kernel<T, true, true><<<grid, kThreads, 0, st>>>(px, py, n, H, W, d);
-  else if (even) dropout_dense_kernel<T, true, false><<<grid, kThreads, 0, st>>>(px, py, n, H, W, d);
-  else if (vec) dropout_dense_kernel<T, false, true><<<grid, kThreads, 0, st>>>(px, py, n, H, W, d);
-  else dropout_dense_kernel<T, false, false><<<grid, kThreads, 0, st>>>(px, py, n, H, W, d);
+  const bool vec = aligned(x, 16);
+  if (even && vec) dropout_dense_kernel<T, true, true><<<grid, kThreads, 0, st>>>(px, py, rows, H, W, log_seg, chunks, per_thread, d);
+  else if (even) dropout_dense_kernel<T, true, false><<<grid, kThreads, 0, st>>>(px, py, rows, H, W, log_seg, chunks, per_thread, d);
+  else if (vec) dropout_dense_kernel<T, false, true><<<grid, kThreads, 0, st>>>(px, py, rows, H, W, log_seg, chunks, per_thread, d);
+  else dropout_dense_kernel<T, false, false><<<grid, kThreads, 0, st>>>(px, py, rows, H, W, log_seg, chunks, per_thread, d);
   return launch_status();
 }
 
@@ -177,7 +232,7 @@ int launch_blocks(const void* x, void* y, const int32_t* idx, const int32_t* nnz
   while ((1 << lh) < BH) ++lh;
   while ((1 << lw) < BW) ++lw;
   const long long pieces = (stride << (lh + lw)) / kPiece;
-  const long long ctas = (pieces + kThreads * kSteps - 1) / (kThreads * kSteps);
+  const long long ctas = (pieces + kThreads * kBatch<T> - 1) / (kThreads * kBatch<T>);
   if (ctas > 0x7fffffffll) return SPARTA_ERR_SHAPE;
   const T* px = static_cast<const T*>(x);
   T* py = static_cast<T*>(y);
@@ -200,11 +255,11 @@ extern "C" int sparta_dropout(const void* x, void* y, int batch, int H, int W, d
   if (!aligned(y, 16) || !aligned(x, dtype == SPARTA_F32 ? 4 : 2) || (rng && !aligned(rng, 8))) return SPARTA_ERR_ALIGN;
   DropoutParams d;
   if (!make_dropout(&d, p, rng, seed, call)) return SPARTA_ERR_BAD_ARG;
-  const long long n = (long long)batch * H * W;
+  const long long rows = (long long)batch * H;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == SPARTA_F32) return launch_dense<float>(x, y, n, H, W, d, st);
-  if (dtype == SPARTA_F16) return launch_dense<__half>(x, y, n, H, W, d, st);
-  return launch_dense<__nv_bfloat16>(x, y, n, H, W, d, st);
+  if (dtype == SPARTA_F32) return launch_dense<float>(x, y, rows, H, W, d, st);
+  if (dtype == SPARTA_F16) return launch_dense<__half>(x, y, rows, H, W, d, st);
+  return launch_dense<__nv_bfloat16>(x, y, rows, H, W, d, st);
 }
 
 extern "C" int sparta_dropout_blocks(const void* x, void* y, const int32_t* bcsr_idx, const int32_t* nnz, int batch, int BH,

@@ -49,33 +49,63 @@ __device__ __forceinline__ PhiloxKey load_philox_key(const DropoutParams& d) {
   return {static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32), call};
 }
 
+// After two of the seven rounds two of the four words depend on (column, batch element) alone, and of the other two's
+// product one factor on (row, batch element) alone: of fourteen products nine depend on both.  Kernels make the row's
+// and the column's share once for as many positions as they can.
+struct PhiloxRow {
+  uint32_t hi, lo;          // of the second round's product, the key in `hi`
+};
+struct PhiloxCol {
+  uint32_t w3, k0, k2, x3;  // round one's fourth word; what the third round's words are combined with; its fourth word
+};
+constexpr uint32_t kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u, kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;
+
+__device__ __forceinline__ PhiloxRow philox_row(const PhiloxKey& key, uint32_t row, uint32_t batch) {
+  const uint32_t x0 = __umulhi(kPhiloxM1, batch) ^ row ^ key.k0;
+  const uint64_t a = static_cast<uint64_t>(kPhiloxM0) * x0;
+  return {static_cast<uint32_t>(a >> 32) ^ (key.k1 + kPhiloxW1), static_cast<uint32_t>(a)};
+}
+__device__ __forceinline__ PhiloxCol philox_col(const PhiloxKey& key, uint32_t g, uint32_t batch) {
+  const uint64_t a1 = static_cast<uint64_t>(kPhiloxM0) * g;
+  const uint64_t b2 = static_cast<uint64_t>(kPhiloxM1) * (static_cast<uint32_t>(a1 >> 32) ^ key.call ^ key.k1);
+  const uint64_t a3 = static_cast<uint64_t>(kPhiloxM0) * (static_cast<uint32_t>(b2 >> 32) ^ (kPhiloxM1 * batch) ^ (key.k0 + kPhiloxW0));
+  return {static_cast<uint32_t>(a1), static_cast<uint32_t>(b2) ^ (key.k0 + 2 * kPhiloxW0),
+          static_cast<uint32_t>(a3 >> 32) ^ (key.k1 + 2 * kPhiloxW1), static_cast<uint32_t>(a3)};
+}
 // eight 16-bit values of columns 8 g .. 8 g + 7, two per word, lower column in the lower half
-__device__ __forceinline__ void philox8(const PhiloxKey& key, uint32_t g, uint32_t row, uint32_t batch, uint32_t (&w)[4]) {
-  uint32_t x0 = g, x1 = row, x2 = batch, x3 = key.call, k0 = key.k0, k1 = key.k1;
+__device__ __forceinline__ void philox8(const PhiloxKey& key, const PhiloxRow& r, const PhiloxCol& c, uint32_t (&w)[4]) {
+  const uint64_t b3 = static_cast<uint64_t>(kPhiloxM1) * (r.hi ^ c.w3);
+  uint32_t x0 = static_cast<uint32_t>(b3 >> 32) ^ c.k0, x1 = static_cast<uint32_t>(b3), x2 = c.k2 ^ r.lo, x3 = c.x3;
 #pragma unroll
-  for (int i = 0; i < 7; ++i) {
-    const uint64_t a = static_cast<uint64_t>(0xD2511F53u) * x0, b = static_cast<uint64_t>(0xCD9E8D57u) * x2;
-    x0 = static_cast<uint32_t>(b >> 32) ^ x1 ^ k0;
+  for (int i = 3; i < 7; ++i) {
+    const uint64_t a = static_cast<uint64_t>(kPhiloxM0) * x0, b = static_cast<uint64_t>(kPhiloxM1) * x2;
+    x0 = static_cast<uint32_t>(b >> 32) ^ x1 ^ (key.k0 + i * kPhiloxW0);
     x1 = static_cast<uint32_t>(b);
-    x2 = static_cast<uint32_t>(a >> 32) ^ x3 ^ k1;
+    x2 = static_cast<uint32_t>(a >> 32) ^ x3 ^ (key.k1 + i * kPhiloxW1);
     x3 = static_cast<uint32_t>(a);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   w[0] = x0; w[1] = x1; w[2] = x2; w[3] = x3;
 }
-
-// bit c: column 8 g + c is kept.  cut = threshold << 16 (threshold < 65536): the upper half of a word is not below the
-// threshold exactly when the word is not below `cut`, the lower half exactly when the word shifted up is not.
-__device__ __forceinline__ uint32_t philox_keep8(const PhiloxKey& key, uint32_t cut, uint32_t g, uint32_t row, uint32_t batch) {
-  uint32_t w[4], bits = 0;
-  philox8(key, g, row, batch, w);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    bits |= ((w[i] << 16) >= cut ? 1u : 0u) << (2 * i);
-    bits |= (w[i] >= cut ? 1u : 0u) << (2 * i + 1);
-  }
-  return bits;
+// the same key in every lane, known to the compiler as such; every lane of the warp calls it
+__device__ __forceinline__ PhiloxKey load_uniform_philox_key(const DropoutParams& d) {
+  const PhiloxKey k = load_philox_key(d);
+  return {__shfl_sync(0xffffffffu, k.k0, 0), __shfl_sync(0xffffffffu, k.k1, 0), __shfl_sync(0xffffffffu, k.call, 0)};
 }
+
+// Bits 15 and 31: the halves of w are not below the halves of t (a threshold below 65536 twice).  Side by side: with
+// the top bits set aside, a subtraction of the lower 15 bits leaves its borrow in place of the top bit, and the result
+// is decided by the top bits or, where they agree, by that.
+__device__ __forceinline__ uint32_t not_below2(uint32_t w, uint32_t t) {
+  const uint32_t d = (w | 0x80008000u) - (t & 0x7fff7fffu);
+  return (w & ~t) | (~(w ^ t) & d);
+}
+// bits 15 and 31 over their halves
+__device__ __forceinline__ uint32_t spread2(uint32_t x) {
+  uint32_t m;
+  asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(m) : "r"(x));  // sign of byte 1, byte 3 over two bytes each
+  return m;
+}
+// The threshold in both halves.  "Everything dropped" (65536) becomes "nothing": its scale is 0.
+__device__ __forceinline__ uint32_t threshold2(const DropoutParams& d) { return (d.threshold & 0xffffu) * 0x00010001u; }
 
 }  // namespace sparta
