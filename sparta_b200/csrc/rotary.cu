@@ -8,8 +8,8 @@
 // product with the position, modulo 2^64, is the angle modulo one turn, exact to position * 2^-65 turns, and its upper
 // half goes to sincospi.
 //
-// Bound by HBM: one read and one write of each element.  A thread holds the angles of V pairs (one 16-byte vector of
-// first and one of second elements) of one token and walks over several heads with them, so that the sines cost a
+// Bound by HBM: one read and one write of each element.  A thread holds the angles of the pairs in one 16-byte vector
+// (interleaved) or in one vector of first and one of second elements of a token and walks over several heads with them, so that the sines cost a
 // few instructions per element; few tokens (a decoding step) are spread over heads instead.  Queries and keys are
 // two entries of one launch (blockIdx.z).  Inputs may have any batch / head / token stride, so the token-major tensor
 // that a projection leaves is turned and brought into the attention's head-major order in one pass.
@@ -51,15 +51,20 @@ __device__ __forceinline__ int64_t position_of(const RotaryTensor& t, int pos64,
                : static_cast<int64_t>(__ldg(static_cast<const int*>(t.positions) + k));
 }
 
-// 16-byte vectors: V elements; half % V == 0, dim % V == 0, addresses and strides multiples of a vector.
+// 16-byte vectors: V elements; the turned part and the head whole vectors, addresses and strides multiples of one.
 template <typename T, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int V = 16 / sizeof(T);
   const RotaryTensor& t = p.t[blockIdx.z];
-  const int turned = p.half / V;                       // units of V pairs
-  const int units = turned + (p.dim - 2 * p.half) / V; // and of V copied elements
-  const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long tokens = (long long)t.batch * t.n;
+  // Units of P pairs, then (in warps of their own) units of V copied elements.  Interleaved pairs take one vector per
+  // unit: with two, a thread's stores were halves of 32-byte sectors (16384 tokens, 40 heads, 96 of 128: 68 us).
+  constexpr int P = INTERLEAVED ? V / 2 : V, kVecs = INTERLEAVED ? 1 : 2, kBatch = 4;  // heads with loads in flight
+  const int turned = p.half / P, copied = (p.dim - 2 * p.half) / V;
+  const long long tokens = (long long)t.batch * t.n, pairs_end = (tokens * turned + 31) / 32 * 32;
+  long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
+  const bool copies = id >= pairs_end;
+  const int units = copies ? copied : turned;
+  if (copies) id -= pairs_end;
   const int h0 = blockIdx.y * p.heads_per_thread;
   if (id >= tokens * units || h0 >= t.heads) return;
   const int h1 = min(h0 + p.heads_per_thread, t.heads);
@@ -69,41 +74,50 @@ __global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_const
   const T* x = static_cast<const T*>(t.x) + b * t.sb + i * t.sn + h0 * t.sh;
   const long long y_head = (long long)t.n * p.dim;
   T* y = static_cast<T*>(t.y) + ((long long)b * t.heads + h0) * y_head + (long long)i * p.dim;
-  if (u >= turned) {
-    const int at = 2 * p.half + (u - turned) * V;
-    for (int h = h0; h < h1; ++h, x += t.sh, y += y_head)
-      *reinterpret_cast<uint4*>(y + at) = __ldg(reinterpret_cast<const uint4*>(x + at));
+  if (copies) {
+    const int at = 2 * p.half + u * V;
+    for (int h = h0; h < h1; h += kBatch) {
+      uint4 v[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (h + j < h1) v[j] = __ldg(reinterpret_cast<const uint4*>(x + (h - h0 + j) * t.sh + at));
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (h + j < h1) *reinterpret_cast<uint4*>(y + (h - h0 + j) * y_head + at) = v[j];
+    }
     return;
   }
-  const int64_t pos = position_of(t, p.pos64, b, i);
-  float c[V], s[V];
+  const int at0 = u * V, at1 = at0 + p.half;
+  float c[P], s[P];
+  for (int h = h0; h < h1; h += kBatch) {
+    __align__(16) T v[kBatch][kVecs * V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) turn_of(__ldg(p.turns + u * V + k), pos, p.magnitude, p.sign, c[k], s[k]);
-  const int at0 = INTERLEAVED ? 2 * u * V : u * V, at1 = INTERLEAVED ? at0 + V : at0 + p.half;
-#pragma unroll 2
-  for (int h = h0; h < h1; ++h, x += t.sh, y += y_head) {
-    __align__(16) T va[V], vb[V];
-    *reinterpret_cast<uint4*>(va) = __ldg(reinterpret_cast<const uint4*>(x + at0));
-    *reinterpret_cast<uint4*>(vb) = __ldg(reinterpret_cast<const uint4*>(x + at1));
-    if constexpr (INTERLEAVED) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        T* v = k < V / 2 ? va : vb;
-        const int o = 2 * (k % (V / 2));
-        const float f0 = to_float(v[o]), f1 = to_float(v[o + 1]);
-        v[o] = from_float<T>(f0 * c[k] - f1 * s[k]);
-        v[o + 1] = from_float<T>(f1 * c[k] + f0 * s[k]);
+    for (int j = 0; j < kBatch; ++j)
+      if (h + j < h1) {
+        const T* src = x + (h - h0 + j) * t.sh;
+        *reinterpret_cast<uint4*>(v[j]) = __ldg(reinterpret_cast<const uint4*>(src + at0));
+        if constexpr (!INTERLEAVED) *reinterpret_cast<uint4*>(v[j] + V) = __ldg(reinterpret_cast<const uint4*>(src + at1));
       }
-    } else {
+    if (h == h0) {  // under the first loads
+      const int64_t pos = position_of(t, p.pos64, b, i);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float f0 = to_float(va[k]), f1 = to_float(vb[k]);
-        va[k] = from_float<T>(f0 * c[k] - f1 * s[k]);
-        vb[k] = from_float<T>(f1 * c[k] + f0 * s[k]);
-      }
+      for (int k = 0; k < P; ++k) turn_of(__ldg(p.turns + u * P + k), pos, p.magnitude, p.sign, c[k], s[k]);
     }
-    *reinterpret_cast<uint4*>(y + at0) = *reinterpret_cast<const uint4*>(va);
-    *reinterpret_cast<uint4*>(y + at1) = *reinterpret_cast<const uint4*>(vb);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (h + j >= h1) break;
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        T& e0 = v[j][INTERLEAVED ? 2 * k : k];
+        T& e1 = v[j][INTERLEAVED ? 2 * k + 1 : V + k];
+        const float f0 = to_float(e0), f1 = to_float(e1);
+        e0 = from_float<T>(f0 * c[k] - f1 * s[k]);
+        e1 = from_float<T>(f1 * c[k] + f0 * s[k]);
+      }
+      T* dst = y + (h - h0 + j) * y_head;
+      *reinterpret_cast<uint4*>(dst + at0) = *reinterpret_cast<const uint4*>(v[j]);
+      if constexpr (!INTERLEAVED) *reinterpret_cast<uint4*>(dst + at1) = *reinterpret_cast<const uint4*>(v[j] + V);
+    }
   }
 }
 
@@ -141,24 +155,28 @@ __global__ void __launch_bounds__(kThreads) rotary_pair_kernel(const __grid_cons
 template <typename T>
 int launch_rotary(RotaryParams& p, int count, int interleaved, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  bool vec = p.half % V == 0 && p.dim % V == 0;
+  const int pairs = interleaved ? V / 2 : V;  // of a thread
+  bool vec = p.half % pairs == 0 && p.dim % V == 0;
   for (int k = 0; k < count; ++k) {
     const RotaryTensor& t = p.t[k];
     vec = vec && aligned(t.x, 16) && aligned(t.y, 16) && t.sb % V == 0 && t.sh % V == 0 && t.sn % V == 0;
   }
-  const int units = vec ? p.half / V + (p.dim - 2 * p.half) / V : p.dim - p.half;
+  const int units = vec ? p.half / pairs + (p.dim - 2 * p.half) / V : p.dim - p.half;
   long long threads = 0, most = 0;
   int heads = 0;
   for (int k = 0; k < count; ++k) {
     const long long one = (long long)p.t[k].batch * p.t[k].n * units;
     threads += one * p.t[k].heads;
-    most = one > most ? one : most;
+    most = one + 31 > most ? one + 31 : most;  // the copies begin at a warp's first lane
     heads = p.t[k].heads > heads ? p.t[k].heads : heads;
   }
-  // heads per thread: as many as leave two threads for every resident slot of the GPU (2048 per SM), at most 8: from
-  // there on the sines are under a tenth of the instructions
-  long long per = threads / (2ll * kNumSMs * 2048);
-  per = per < 1 ? 1 : per > 8 ? 8 : per;
+  // heads per thread: as many as leave half a thread for every resident slot of the GPU (2048 per SM), so that a token's
+  // sines serve many heads; with four heads' loads in flight that many threads keep HBM busy (B4 H16 S4096 D64 fp16:
+  // 28.4 us with up to 8 heads taken one after the other, 20.8 us = 99 % of the measured HBM rate)
+  long long per = threads / (kNumSMs * 1024ll);
+  if (per > 8) per = 8;  // longer loops leave the last wave of blocks half empty (16384 tokens, 40 heads: 71 us with up to 32, 55 us)
+  per = per < 1 ? 1 : per > heads ? heads : per;
+  per = (heads + (heads + per - 1) / per - 1) / ((heads + per - 1) / per);  // even shares
   while ((heads + per - 1) / per > 65535) per *= 2;  // grid.y
   p.heads_per_thread = static_cast<int>(per);
   const long long gx = (most + kThreads - 1) / kThreads;
