@@ -3,8 +3,9 @@
 There is no CPU or eager fallback: when the shared library is missing, ``lib()`` raises, and every
 operator of this package goes through ``lib()``.
 """
-import contextlib
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from typing import Optional
@@ -12,6 +13,7 @@ from typing import Optional
 import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'lib', 'libsparta_b200.so')
+TORCH_OPS_PATH = os.path.join(os.path.dirname(LIB_PATH), '_torch_ops.so')
 
 OK = 0
 F32, F16, BF16 = 0, 1, 2
@@ -132,6 +134,24 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
+_TORCH_OPS = None
+
+
+def torch_ops():
+    """The autograd functions of ``csrc/torch_ops.cpp`` (``dropout``, ``rotary``, ``attention``); raises when they have not
+    been built."""
+    global _TORCH_OPS
+    if _TORCH_OPS is None:
+        if not os.path.exists(TORCH_OPS_PATH):
+            raise RuntimeError(f'{TORCH_OPS_PATH} is missing: build it with `python -m sparta_b200.csrc.build`')
+        loader = importlib.machinery.ExtensionFileLoader('_torch_ops', TORCH_OPS_PATH)
+        spec = importlib.util.spec_from_loader('_torch_ops', loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        _TORCH_OPS = module
+    return _TORCH_OPS
+
+
 class SpartaError(RuntimeError):
     def __init__(self, status: int, where: str):
         text = lib().sparta_status_string(status).decode()
@@ -147,14 +167,6 @@ def check(status: int, where: str):
 def stream_ptr(device=None) -> int:
     index = device.index if isinstance(device, torch.device) else device
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
-
-
-_SAME_DEVICE = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """Context in which ``device`` is current; free of charge when it is already."""
-    return _SAME_DEVICE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

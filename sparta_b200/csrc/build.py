@@ -1,4 +1,5 @@
-"""Build ``libsparta_b200.so`` (the C-ABI library of ``include/sparta_b200.h``) for sm_100a.
+"""Build ``libsparta_b200.so`` (the C-ABI library of ``include/sparta_b200.h``) for sm_100a, and on top of it
+``_torch_ops.so``, the training operators as torch autograd functions (``torch_ops.cpp``).
 
 Usage: ``python -m sparta_b200.csrc.build [--force] [--verbose]``.  Objects go to ``build/`` at the
 repository root, the shared library next to the Python package (``sparta_b200/lib``) so that a
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 CSRC = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(CSRC)
@@ -17,6 +19,7 @@ ROOT = os.path.dirname(PKG)
 OBJ_DIR = os.path.join(ROOT, 'build', 'obj')
 LIB_DIR = os.path.join(PKG, 'lib')
 LIB_PATH = os.path.join(LIB_DIR, 'libsparta_b200.so')
+TORCH_OPS_PATH = os.path.join(LIB_DIR, '_torch_ops.so')
 
 NVCC_FLAGS = [
     '-gencode', 'arch=compute_100a,code=sm_100a',
@@ -61,12 +64,44 @@ def _compile(src: str, force: bool, verbose: bool) -> str:
     return obj
 
 
+def _compile_torch_ops(force: bool, verbose: bool) -> str:
+    from torch.utils import cpp_extension
+    obj, path = os.path.join(OBJ_DIR, 'torch_ops.o'), os.path.join(CSRC, 'torch_ops.cpp')
+    header = os.path.join(ROOT, 'include', 'sparta_b200.h')
+    if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(path), os.path.getmtime(header)):
+        return obj
+    includes = [*cpp_extension.include_paths('cuda'), sysconfig.get_paths()['include']]
+    cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-DTORCH_EXTENSION_NAME=_torch_ops', '-DTORCH_API_INCLUDE_EXTENSION_H',
+           *[f'-isystem{d}' for d in includes], '-c', path, '-o', obj]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or res.returncode != 0:
+        sys.stderr.write(f'$ {" ".join(cmd)}\n{res.stdout}{res.stderr}')
+    if res.returncode != 0:
+        raise RuntimeError('g++ failed on torch_ops.cpp')
+    return obj
+
+
+def _link_torch_ops(obj: str, force: bool):
+    from torch.utils import cpp_extension
+    if not force and os.path.exists(TORCH_OPS_PATH) and os.path.getmtime(TORCH_OPS_PATH) >= os.path.getmtime(obj):
+        return
+    dirs = cpp_extension.library_paths('cuda')
+    cmd = ['g++', '-shared', '-o', TORCH_OPS_PATH, obj, *[f'-L{d}' for d in (LIB_DIR, *dirs)], '-lsparta_b200', '-lc10', '-lc10_cuda',
+           '-ltorch_cpu', '-ltorch_cuda', '-ltorch', '-ltorch_python', '-Wl,-rpath,$ORIGIN', f'-Wl,-rpath,{dirs[0]}']
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError('linking _torch_ops.so failed')
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every .cu of this directory and link the shared library; returns its path."""
+    """Compile every .cu of this directory and link the shared library, then the torch functions on top of it; returns
+    the library's path."""
     os.makedirs(OBJ_DIR, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     srcs = _sources()
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as pool:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as pool:
+        torch_ops = pool.submit(_compile_torch_ops, force, verbose)
         objs = list(pool.map(lambda s: _compile(s, force, verbose), srcs))
     newest = max(os.path.getmtime(o) for o in objs)
     if force or not os.path.exists(LIB_PATH) or os.path.getmtime(LIB_PATH) < newest:
@@ -76,6 +111,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError('linking libsparta_b200.so failed')
+    _link_torch_ops(torch_ops.result(), force)
     return LIB_PATH
 
 

@@ -37,37 +37,6 @@ FUSED_DTYPES = (torch.float16, torch.bfloat16)
 FUSED_MAX_BLOCKS = 1024
 
 
-def _rows(x: torch.Tensor, n: int) -> torch.Tensor:
-    """(..., n, E) as the contiguous, 16-byte aligned (heads, n, E) that the fused kernels read."""
-    x = x.reshape(-1, n, x.shape[-1]).contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
-
-
-class _FusedAttentionFunc(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, op: 'SparseAttention', query, key, value, p: float, rng: Optional[torch.Tensor], seed: int, call: int):
-        ctx.op, ctx.indexes, ctx.dropout = op, op._sparse_port.indexes, (p, seed, call)
-        ctx.shapes = query.shape, key.shape, value.shape
-        q, k, v = (_rows(x.detach(), n) for x, n in ((query, op._Nt), (key, op._Ns), (value, op._Ns)))
-        out, lse, mask = op._fused_train_forward(q, k, v, query.shape, p, DropoutKey(rng, seed, call))
-        # an element mask is read again: autograd refuses if it was rewritten in place since
-        ctx.save_for_backward(q, k, v, out, lse, mask, rng)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        q, k, v, out, lse, mask, rng = ctx.saved_tensors
-        p, seed, call = ctx.dropout
-        want_q, want_kv = ctx.needs_input_grad[1], ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
-        grads = ctx.op._fused_train_backward(q, k, v, out, lse, _rows(grad.detach(), q.shape[1]), ctx.indexes, mask, p,
-                                             DropoutKey(rng, seed, call), want_q, want_kv)
-        dq, dk, dv = (g if g is None else g.view(shape) for g, shape in zip(grads, ctx.shapes))
-        return (None, dq, dk if ctx.needs_input_grad[2] else None, dv if ctx.needs_input_grad[3] else None,
-                None, None, None, None)
-
-
 class SparseAttention(OperatorBase):
     r"""Sparse attention :math:`\text{Softmax}(Q K^T) V`.
 
@@ -120,7 +89,7 @@ class SparseAttention(OperatorBase):
         p, numbers = 0.0, DropoutKey(None, 0, 0)
         if self._dropout is not None and self.training and self._dropout.p > 0.0:
             _lib.require_cuda(query)
-            p, numbers = self._dropout.p, self._dropout._counter.next(rng, query)
+            p, numbers = self._dropout.p, self._dropout._counter.next(rng)
         if self.ready and self._use_fused and (self._fused_request is True or query.dtype in FUSED_DTYPES):
             group = self._check_heads(query, key, value)
             wants_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, value))
@@ -128,7 +97,7 @@ class SparseAttention(OperatorBase):
                 return self._fused_forward(query.detach(), key.detach(), value.detach())
             # the fused backward pass lists the blocks along both sides
             if not wants_grad or self._fused_request is True or self._Nt // FUSED_BLOCK <= FUSED_MAX_BLOCKS:
-                return _FusedAttentionFunc.apply(self, query, key, value, p, *numbers)
+                return self._fused_train(query, key, value, p, numbers)
         shape = query.shape
         if query.dim() != 3 or key.shape[:-2] != query.shape[:-2]:
             query, key, value = self._flat_heads(query, key, value)
@@ -160,49 +129,13 @@ class SparseAttention(OperatorBase):
             key, value = key.repeat_interleave(group, 0), value.repeat_interleave(group, 0)
         return query, key, value
 
-    def _train_args(self, q, k, v, out, lse, indexes, mask, p: float, numbers: DropoutKey) -> '_lib.AttnTrainArgs':
-        if self._attn_status is None or self._attn_status.device != q.device:
-            self._attn_status = torch.zeros(4, dtype=torch.int32, device=q.device)
-        return _lib.AttnTrainArgs(  # in the order of its fields
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), None, None, None, None, None, 0,
-            indexes.row_ptr.data_ptr(), indexes.bcsr_buf.data_ptr(), _lib.ptr(mask), _lib.ptr(numbers.rng),
-            numbers.seed & 0xffffffffffffffff, numbers.call & 0xffffffff, indexes.block_nnz, self._attn_status.data_ptr(), p, self._scale,
-            q.shape[0], k.shape[0], self._Nt, self._Ns, q.shape[2], FUSED_BLOCK, _lib.dtype_code(q))
-
-    def _raise_on_status(self):
-        if self.check_status and any(self.fused_status()):
-            raise RuntimeError(f'fused sparse attention: a bounded wait ran out on the device, status words '
-                               f'{self.fused_status()}; the output is invalid')
-
-    def _fused_train_forward(self, q, k, v, shape, p: float, numbers: DropoutKey):
-        _lib.require_cuda(q, k, v)
+    def _fused_train(self, query, key, value, p: float, numbers: DropoutKey) -> torch.Tensor:
         idx = self._sparse_port.indexes
-        mask = None if idx.block_uniform else idx.raw_mask
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        if out.numel() > 0:
-            with _lib.on_device(q.device):
-                _lib.check(_lib.lib().sparta_attn_train_fwd(self._train_args(q, k, v, out, lse, idx, mask, p, numbers),
-                                                            _lib.stream_ptr(q.device)), 'sparta_attn_train_fwd')
-            self._raise_on_status()
-        return out, lse, mask
-
-    def _fused_train_backward(self, q, k, v, out, lse, grad, indexes, mask, p: float, numbers: DropoutKey,
-                              want_q: bool, want_kv: bool):
-        dq = torch.empty_like(q) if want_q else None
-        dk, dv = (torch.empty_like(k), torch.empty_like(v)) if want_kv else (None, None)
-        if not (want_q or want_kv):
-            return dq, dk, dv
-        L = _lib.lib()
-        ws = torch.empty(L.sparta_attn_train_bwd_workspace_bytes(q.shape[0], k.shape[0], self._Nt, self._Ns, q.shape[2],
-                                                                 indexes.block_nnz), dtype=torch.uint8, device=q.device)
-        args = self._train_args(q, k, v, out, lse, indexes, mask, p, numbers)
-        args.dO, args.dQ, args.dK, args.dV = grad.data_ptr(), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
-        with _lib.on_device(q.device):
-            _lib.check(L.sparta_attn_train_bwd(args, _lib.stream_ptr(q.device)), 'sparta_attn_train_bwd')
-        self._raise_on_status()
-        return dq, dk, dv
+        if self._attn_status is None or self._attn_status.device != query.device:
+            self._attn_status = torch.zeros(4, dtype=torch.int32, device=query.device)
+        return _lib.torch_ops().attention(
+            query, key, value, idx.row_ptr, idx.bcsr_buf, None if idx.block_uniform else idx.raw_mask, self._attn_status,
+            numbers.rng, p, self._scale, numbers.seed, numbers.call, idx.block_nnz, self._Nt, self._Ns, self.check_status)
 
     def forward_gathered(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                          out: torch.Tensor, copies: List[int]) -> torch.Tensor:

@@ -23,11 +23,10 @@ def check_probability(p: float) -> float:
     return p
 
 
-def check_rng(rng: torch.Tensor, x: torch.Tensor):
-    if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous():
-        raise ValueError('rng has to be a contiguous int64 tensor of two numbers (seed, call number)')
-    if rng.device != x.device:
-        raise ValueError(f'rng is on {rng.device}, the input on {x.device}')
+def signed64(seed: int) -> int:
+    """The lower 64 bits of a seed as a signed number."""
+    seed &= (1 << 64) - 1
+    return seed - (1 << 64) if seed >> 63 else seed
 
 
 class _Counter(object):
@@ -37,71 +36,29 @@ class _Counter(object):
         self.seed = int(torch.randint(0, 1 << 62, (), dtype=torch.int64)) if seed is None else int(seed)
         self.calls = 0
 
-    def next(self, rng: Optional[torch.Tensor], x: torch.Tensor) -> DropoutKey:
+    def next(self, rng: Optional[torch.Tensor]) -> DropoutKey:
         if rng is not None:
-            check_rng(rng, x)
             return DropoutKey(rng, 0, 0)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError('a captured graph would repeat the same dropout at every replay: pass rng, an int64 '
                                'tensor (seed, call number) on the GPU, and rewrite it between replays')
-        key = DropoutKey(None, self.seed, self.calls)
+        key = DropoutKey(None, signed64(self.seed), self.calls)
         self.calls += 1
         return key
 
 
-def _launch(x: torch.Tensor, p: float, rng: Optional[torch.Tensor], seed: int, call: int,
-            indexes: Optional[BCSIndexes]) -> torch.Tensor:
-    x = x.contiguous()
-    y = torch.empty_like(x)
-    n = x.numel()
-    if n == 0:
-        return y
-    device, shape = x.device, x.shape
-    with _lib.on_device(device):
-        if indexes is None:
-            W = shape[-1] if shape else 1
-            H = shape[-2] if len(shape) > 1 else 1
-            _lib.check(_lib.lib().sparta_dropout(
-                x.data_ptr(), y.data_ptr(), n // (H * W), H, W, p, _lib.ptr(rng), seed & 0xffffffffffffffff,
-                call & 0xffffffff, _lib.dtype_code(x), _lib.stream_ptr(device)), 'sparta_dropout')
-        else:
-            _lib.check(_lib.lib().sparta_dropout_blocks(
-                x.data_ptr(), y.data_ptr(), indexes.bcsr_buf.data_ptr(), indexes.nnz_dev.data_ptr(), n // shape[-1],
-                indexes.block_H, indexes.block_W, indexes.val_stride_blocks, p, _lib.ptr(rng),
-                seed & 0xffffffffffffffff, call & 0xffffffff, _lib.dtype_code(x), _lib.stream_ptr(device)),
-                'sparta_dropout_blocks')
-    return y
-
-
-class SparseDropoutFunc(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, x: torch.Tensor, p: float, rng: Optional[torch.Tensor], seed: int, call: int,
-                indexes: Optional[BCSIndexes]):
-        ctx.p, ctx.numbers, ctx.indexes = p, (seed, call), indexes
-        ctx.save_for_backward(rng)  # rewritten before the backward pass: autograd refuses
-        return _launch(x, p, rng, seed, call, indexes)
-
-    @staticmethod
-    def backward(ctx, grad: torch.Tensor):
-        rng, = ctx.saved_tensors
-        # linear: the gradient's own gradient is the same operator; the plain launch skips autograd's bookkeeping
-        run = SparseDropoutFunc.apply if torch.is_grad_enabled() else _launch
-        return run(grad, ctx.p, rng, *ctx.numbers, ctx.indexes), None, None, None, None, None
-
-
 def sparse_dropout(x: torch.Tensor, p: float, key: DropoutKey, indexes: Optional[BCSIndexes] = None) -> torch.Tensor:
     """Dropout of ``x`` with the random numbers of ``key``; see ``SparseDropout``."""
-    _lib.require_cuda(x)
-    _lib.dtype_code(x)
-    if indexes is not None:
-        if indexes.batched or not indexes.BCSR:
-            raise ValueError('dropout of block values needs the BCSR indexes of one 2-D mask')
-        if indexes.block_W < 8:
-            raise ValueError(f'dropout of block values needs blocks at least 8 wide, got {indexes.block_W}')
-        if x.dim() == 0 or x.shape[-1] != indexes.val_stride_blocks * indexes.block_H * indexes.block_W:
-            raise ValueError(f'the input of shape {tuple(x.shape)} does not hold the block values of these indexes')
-    return SparseDropoutFunc.apply(x, p, key.rng, key.seed, key.call, indexes)
+    if indexes is None:
+        return _lib.torch_ops().dropout(x, p, key.rng, key.seed, key.call, None, None, 0, 0, 0)
+    if indexes.batched or not indexes.BCSR:
+        raise ValueError('dropout of block values needs the BCSR indexes of one 2-D mask')
+    if indexes.block_W < 8:
+        raise ValueError(f'dropout of block values needs blocks at least 8 wide, got {indexes.block_W}')
+    if x.dim() == 0 or x.shape[-1] != indexes.val_stride_blocks * indexes.block_H * indexes.block_W:
+        raise ValueError(f'the input of shape {tuple(x.shape)} does not hold the block values of these indexes')
+    return _lib.torch_ops().dropout(x, p, key.rng, key.seed, key.call, indexes.bcsr_buf, indexes.nnz_dev, indexes.block_H,
+                                    indexes.block_W, indexes.val_stride_blocks)
 
 
 class SparseDropout(torch.nn.Module):
@@ -134,7 +91,7 @@ class SparseDropout(torch.nn.Module):
         if not self.training or self.p == 0.0:
             return x
         _lib.require_cuda(x)
-        return sparse_dropout(x, self.p, self._counter.next(rng, x), indexes)
+        return sparse_dropout(x, self.p, self._counter.next(rng), indexes)
 
     def get_extra_state(self):
         return {'seed': self._counter.seed, 'calls': self._counter.calls}
