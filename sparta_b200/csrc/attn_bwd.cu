@@ -60,18 +60,21 @@ struct BwdParams {
   const uint8_t* present;   // [Nt / 64, present_pitch]: block kept (built by the first kernel)
   const float* neg_lse;     // [heads, Nt]: -lse * log2(e), -inf for a row without any score
   const float* neg_delta;   // [heads, Nt]
-  void* out1;               // dQ, or dK
-  void* out2;               // dV
   int Nt, Ns, heads, kv_heads, group;
   int present_pitch;
-  int by_head;              // launch order: tiles of a head together
-  int split;                // CTAs per tile at most, see the kernel
-  int split_steps;          // steps that one of them should take
-  float* partial;           // [heads, tiles, split, 128, columns of the sums], where a tile is split
-  uint32_t* tickets;        // [heads, tiles], zero
   float scale, scale_log2;
   int32_t* status;
   DropoutParams drop;
+};
+
+struct PassParams {         // of one of the two passes
+  void* out1;               // dQ, or dK
+  void* out2;               // dV
+  int by_head;              // launch order: tiles of a head together
+  int split;                // CTAs per tile at most
+  int split_steps;          // steps that one of them should take
+  float* partial;           // [heads, tiles, split, columns of the sums, 128], where a tile is split
+  uint32_t* tickets;        // [heads, tiles], zero
 };
 
 template <bool DKV, int D>
@@ -125,30 +128,42 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
 }
 
 // The negated delta and log-sum-exp of every query row; the blocks kept, as bytes, for the pass that walks columns.
-// Bound by the read of O and dO.  A row is D / 8 lanes of 16 bytes.
+// Bound by the read of O and dO.  A row is D / 8 lanes of 16 bytes; four rows' loads are in flight per thread.
+constexpr int kPrepRows = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(256)
 attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const float* __restrict__ lse, float* __restrict__ neg_lse,
                      float* __restrict__ neg_delta, uint8_t* __restrict__ present, const int32_t* __restrict__ row_ptr,
                      const int32_t* __restrict__ idx, long long rows, int nbr, int nbc, int pitch,
                      uint32_t* __restrict__ tickets, long long n_tickets) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 8, kStep = 256 / kLanes;
   const int lane = threadIdx.x % kLanes;
-  const long long row = (long long)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  float sum = 0.f;
-  if (row < rows) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(O + row * D) + lane);
-    const uint4 b = __ldg(reinterpret_cast<const uint4*>(dO + row * D) + lane);
-    const T* x = reinterpret_cast<const T*>(&a);
-    const T* y = reinterpret_cast<const T*>(&b);
+  const long long row0 = (long long)blockIdx.x * (kPrepRows * kStep) + threadIdx.x / kLanes;
+  uint4 a[kPrepRows], b[kPrepRows];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(to_float(x[i]), to_float(y[i]), sum);
+  for (int k = 0; k < kPrepRows; ++k) {
+    const long long row = row0 + k * kStep;
+    a[k] = b[k] = make_uint4(0, 0, 0, 0);
+    if (row < rows) {
+      a[k] = __ldg(reinterpret_cast<const uint4*>(O + row * D) + lane);
+      b[k] = __ldg(reinterpret_cast<const uint4*>(dO + row * D) + lane);
+    }
   }
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (row < rows && lane == 0) {
-    neg_delta[row] = -sum;
-    neg_lse[row] = lse[row] > -INFINITY ? lse[row] * -1.4426950408889634f : -INFINITY;
+  for (int k = 0; k < kPrepRows; ++k) {
+    const long long row = row0 + k * kStep;
+    const T* x = reinterpret_cast<const T*>(&a[k]);
+    const T* y = reinterpret_cast<const T*>(&b[k]);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(to_float(x[i]), to_float(y[i]), sum);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (row < rows && lane == 0) {
+      neg_delta[row] = -sum;
+      // (a NaN stays one, so that it reaches the gradients)
+      neg_lse[row] = lse[row] == -INFINITY ? -INFINITY : lse[row] * -1.4426950408889634f;
+    }
   }
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n_tickets; i += (long long)gridDim.x * 256) tickets[i] = 0;
   __shared__ uint8_t kept[kMaxBlocks];
@@ -168,9 +183,8 @@ attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const fl
 // SPLIT: several CTAs may share a tile.  A variant of its own, because the other one keeps its registers for the steps
 // (B4 H16 S4096 D64, which does not split: 509 us with the code for it, 483 us without).
 template <bool DKV, int D, int FMT, bool MASK, bool DROP, bool SPLIT>
-__global__ void __launch_bounds__(BwdCfg<DKV, D>::kThreads, BwdCfg<DKV, D>::kCtasPerSM)
-attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant__ CUtensorMap tm_a2,
-                const __grid_constant__ CUtensorMap tm_b1, const __grid_constant__ CUtensorMap tm_b2, const BwdParams p) {
+__device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtensorMap& tm_a2, const CUtensorMap& tm_b1,
+                                         const CUtensorMap& tm_b2, const BwdParams& p, const PassParams& pass, int block) {
   using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
   using C = BwdCfg<DKV, D>;
   constexpr int kSBuf = C::kSBuf, kStages = C::kStages, kChunks = C::kChunks, kThreads = C::kThreads;
@@ -205,18 +219,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
   const int heads = DKV ? p.kv_heads : p.heads;
   const int tiles = (rows + kTileM - 1) / kTileM;
   int head, tile;                                      // and the CTA's part of the tile
-  if (!p.by_head) {  // the first tiles of all heads first: with global tokens they are the longest
-    tile = blockIdx.x / heads;
-    head = blockIdx.x - tile * heads;
+  if (!pass.by_head) {  // the first tiles of all heads first: with global tokens they are the longest
+    tile = block / heads;
+    head = block - tile * heads;
   } else {
-    const int per_head = SPLIT ? tiles * p.split : tiles;
-    head = blockIdx.x / per_head;
-    tile = blockIdx.x - head * per_head;
+    const int per_head = SPLIT ? tiles * pass.split : tiles;
+    head = block / per_head;
+    tile = block - head * per_head;
   }
   int part = 0;
   if constexpr (SPLIT) {
-    part = tile % p.split;
-    tile /= p.split;
+    part = tile % pass.split;
+    tile /= pass.split;
   }
   const int blk0 = tile * 2;                           // first of the tile's two blocks
   const int nbr = p.Nt / kBlk, nbc = p.Ns / kBlk;
@@ -285,7 +299,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
   // last one to finish adds them in their order.
   int parts = 1, step0 = 0, steps = all_steps, h0 = 0, k0 = 0;  // step = h * pairs + k
   if constexpr (SPLIT) {
-    parts = min(p.split, max(1, (all_steps + p.split_steps / 2) / p.split_steps));
+    parts = min(pass.split, max(1, (all_steps + pass.split_steps / 2) / pass.split_steps));
     if (part >= parts) {
       if (warp == kWarpMma) tmem_dealloc<C::kTmemCols>(tmem_base);
       return;
@@ -597,7 +611,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
     const long long tile_id = (long long)head * tiles + tile;
     // partial sums: [piece][float4 of the piece][row], so that a warp's accesses are contiguous
     auto partial_at = [&](int of, int piece) {
-      return reinterpret_cast<float4*>(p.partial) + ((tile_id * p.split + of) * kPieces + piece) * (8 * kTileM) + row;
+      return reinterpret_cast<float4*>(pass.partial) + ((tile_id * pass.split + of) * kPieces + piece) * (8 * kTileM) + row;
     };
     auto load_piece = [&](int piece, float (&v)[32]) {
       if (steps > 0 && ok) {
@@ -614,7 +628,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
     auto store_piece = [&](int piece, const float (&v)[32]) {
       const bool second = piece >= D / 32;             // dV
       const float f = second ? (DROP ? up : 1.f) : p.scale;
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(second ? p.out2 : p.out1) + (a_row0 + row) * D + (piece % (D / 32)) * 32);
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(second ? pass.out2 : pass.out1) + (a_row0 + row) * D + (piece % (D / 32)) * 32);
       if (inside) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -638,7 +652,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
       }
       __threadfence();
       named_barrier_sync(1, kScoreWarps * 32);
-      if (threadIdx.x == 0) *s_last = atomicAdd(p.tickets + tile_id, 1u) == static_cast<uint32_t>(parts - 1);
+      if (threadIdx.x == 0) *s_last = atomicAdd(pass.tickets + tile_id, 1u) == static_cast<uint32_t>(parts - 1);
       named_barrier_sync(1, kScoreWarps * 32);
       if (*s_last) {  // the others' sums are in L2
         __threadfence();
@@ -667,6 +681,23 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_a1, const __grid_constant
   }
 }
 
+// Tensor maps by tensor and box height: as resident tiles and as streamed blocks.
+struct BwdMaps {
+  CUtensorMap q_tile, do_tile, k_tile, v_tile, q_block, do_block, k_block, v_block;
+};
+
+// Both passes in one launch, the blocks of the dK, dV pass first (its tiles take longer): nothing of one needs anything
+// of the other, and the last blocks of the first run beside the first of the second.
+template <int D, int FMT, bool MASK, bool DROP, bool SPLIT>
+__global__ void __launch_bounds__(BwdCfg<true, D>::kThreads, BwdCfg<true, D>::kCtasPerSM)
+attn_bwd_kernel(const __grid_constant__ BwdMaps m, const __grid_constant__ BwdParams p, const __grid_constant__ PassParams kv,
+                const __grid_constant__ PassParams q, int kv_blocks) {
+  static_assert(BwdCfg<true, D>::kThreads == BwdCfg<false, D>::kThreads, "one launch, one block size");
+  const int block = blockIdx.x;
+  if (block < kv_blocks) bwd_pass<true, D, FMT, MASK, DROP, SPLIT>(m.k_tile, m.v_tile, m.q_block, m.do_block, p, kv, block);
+  else bwd_pass<false, D, FMT, MASK, DROP, SPLIT>(m.q_tile, m.do_tile, m.k_block, m.v_block, p, q, block - kv_blocks);
+}
+
 int rows_map(CUtensorMap* map, const void* base, int dtype, int D, long long rows, uint32_t box_rows) {
   const uint64_t dims[2] = {(uint64_t)D, (uint64_t)rows}, strides[1] = {(uint64_t)D * 2};
   const uint32_t box[2] = {64, box_rows};
@@ -682,7 +713,7 @@ struct PassPlan {
   size_t partial_bytes;
 };
 constexpr int kMinSteps = 12, kMaxSplit = 16;
-constexpr size_t kMaxPartialBytes = size_t(256) << 20;
+constexpr size_t kMaxPartialBytes = size_t(128) << 20;  // of a pass
 
 template <bool DKV, int D>
 PassPlan plan_pass(int heads, int kv_heads, int Nt, int Ns, long long nnz) {
@@ -706,26 +737,11 @@ PassPlan plan_pass(int heads, int kv_heads, int Nt, int Ns, long long nnz) {
   return plan;
 }
 
-template <bool DKV, int D, int FMT, bool MASK, bool DROP, bool SPLIT>
-int launch_pass(const CUtensorMap& a1, const CUtensorMap& a2, const CUtensorMap& b1, const CUtensorMap& b2, BwdParams p,
-                const PassPlan& plan, cudaStream_t st) {
-  using C = BwdCfg<DKV, D>;
-  auto kern = attn_bwd_kernel<DKV, D, FMT, MASK, DROP, SPLIT>;
-  static SmemAttrOnce attr;
-  if (cudaError_t e = attr.ensure(kern, C::kSmem); e != cudaSuccess) return static_cast<int>(e);
-  const long long ctas = (long long)(DKV ? p.kv_heads : p.heads) * plan.tiles * plan.split;
-  if (ctas > 0x7fffffffll) return SPARTA_ERR_SHAPE;
-  p.split = plan.split;
-  p.split_steps = plan.split_steps;
-  kern<<<static_cast<unsigned>(ctas), C::kThreads, C::kSmem, st>>>(a1, a2, b1, b2, p);
-  return launch_status();
-}
-
 int present_pitch(int Ns) { return (Ns / kBlk + 1) & ~1; }
 size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
 
 struct Workspace {
-  size_t neg_lse, neg_delta, present, tickets_q, tickets_kv, partial, total;
+  size_t neg_lse, neg_delta, present, tickets_q, tickets_kv, partial_q, partial_kv, total;
   long long n_tickets;
   PassPlan q, kv;
 };
@@ -740,8 +756,9 @@ Workspace lay_out(int heads, int kv_heads, int Nt, int Ns, long long nnz) {
   w.present = w.neg_delta + round16(sizeof(float) * (size_t)heads * Nt);
   w.tickets_q = w.present + round16((size_t)(Nt / kBlk) * present_pitch(Ns));
   w.tickets_kv = w.tickets_q + sizeof(uint32_t) * (size_t)heads * w.q.tiles;
-  w.partial = w.tickets_q + round16(sizeof(uint32_t) * (size_t)w.n_tickets);
-  w.total = w.partial + (w.q.partial_bytes > w.kv.partial_bytes ? w.q.partial_bytes : w.kv.partial_bytes);  // one pass at a time
+  w.partial_q = w.tickets_q + round16(sizeof(uint32_t) * (size_t)w.n_tickets);
+  w.partial_kv = w.partial_q + w.q.partial_bytes;
+  w.total = w.partial_kv + w.kv.partial_bytes;
   return w;
 }
 
@@ -754,42 +771,47 @@ int launch_bwd(const AttnArgs& a, BwdParams p, cudaStream_t st) {
   float* neg_delta = reinterpret_cast<float*>(ws + w.neg_delta);
   uint32_t* tickets_q = reinterpret_cast<uint32_t*>(ws + w.tickets_q);
   p.neg_lse = neg_lse; p.neg_delta = neg_delta; p.present = ws + w.present;
-  p.partial = reinterpret_cast<float*>(ws + w.partial);
   p.present_pitch = present_pitch(a.Ns);
   const long long q_rows = (long long)a.heads * a.Nt, k_rows = (long long)a.kv_heads * a.Ns;
-  const long long ctas = (q_rows + 2048 / D - 1) / (2048 / D);
-  attn_bwd_prep_kernel<T, D><<<static_cast<unsigned>(ctas), 256, 0, st>>>(
+  constexpr int kRowsPerBlock = kPrepRows * 2048 / D;
+  const long long prep_ctas = (q_rows + kRowsPerBlock - 1) / kRowsPerBlock;
+  attn_bwd_prep_kernel<T, D><<<static_cast<unsigned>(prep_ctas), 256, 0, st>>>(
       static_cast<const T*>(a.O), static_cast<const T*>(a.dO), a.lse, neg_lse, neg_delta, ws + w.present, a.row_ptr, a.idx, q_rows,
       a.Nt / kBlk, a.Ns / kBlk, p.present_pitch, tickets_q, w.n_tickets);
   if (int rc = launch_status(); rc != SPARTA_OK) return rc;
-  CUtensorMap a1, a2, b1, b2;
-  if (a.dK) {
-    int rc = rows_map(&a1, a.K, a.dtype, D, k_rows, kTileM);
-    if (rc == SPARTA_OK) rc = rows_map(&a2, a.V, a.dtype, D, k_rows, kTileM);
-    if (rc == SPARTA_OK) rc = rows_map(&b1, a.Q, a.dtype, D, q_rows, kBlk);
-    if (rc == SPARTA_OK) rc = rows_map(&b2, a.dO, a.dtype, D, q_rows, kBlk);
-    if (rc != SPARTA_OK) return rc;
-    p.out1 = a.dK; p.out2 = a.dV;
-    p.by_head = kv_exceeds_l2(a.heads, a.Nt, D);
-    p.tickets = reinterpret_cast<uint32_t*>(ws + w.tickets_kv);
-    rc = w.kv.split > 1 ? launch_pass<true, D, FMT, MASK, DROP, true>(a1, a2, b1, b2, p, w.kv, st)
-                        : launch_pass<true, D, FMT, MASK, DROP, false>(a1, a2, b1, b2, p, w.kv, st);
-    if (rc != SPARTA_OK) return rc;
-  }
-  if (a.dQ) {
-    int rc = rows_map(&a1, a.Q, a.dtype, D, q_rows, kTileM);
-    if (rc == SPARTA_OK) rc = rows_map(&a2, a.dO, a.dtype, D, q_rows, kTileM);
-    if (rc == SPARTA_OK) rc = rows_map(&b1, a.K, a.dtype, D, k_rows, kBlk);
-    if (rc == SPARTA_OK) rc = rows_map(&b2, a.V, a.dtype, D, k_rows, kBlk);
-    if (rc != SPARTA_OK) return rc;
-    p.out1 = a.dQ; p.out2 = nullptr;
-    p.by_head = kv_exceeds_l2(a.kv_heads, a.Ns, D);
-    p.tickets = tickets_q;
-    rc = w.q.split > 1 ? launch_pass<false, D, FMT, MASK, DROP, true>(a1, a2, b1, b2, p, w.q, st)
-                       : launch_pass<false, D, FMT, MASK, DROP, false>(a1, a2, b1, b2, p, w.q, st);
-    if (rc != SPARTA_OK) return rc;
-  }
-  return SPARTA_OK;
+  BwdMaps m;
+  int rc = rows_map(&m.q_tile, a.Q, a.dtype, D, q_rows, kTileM);
+  if (rc == SPARTA_OK) rc = rows_map(&m.do_tile, a.dO, a.dtype, D, q_rows, kTileM);
+  if (rc == SPARTA_OK) rc = rows_map(&m.k_tile, a.K, a.dtype, D, k_rows, kTileM);
+  if (rc == SPARTA_OK) rc = rows_map(&m.v_tile, a.V, a.dtype, D, k_rows, kTileM);
+  if (rc == SPARTA_OK) rc = rows_map(&m.q_block, a.Q, a.dtype, D, q_rows, kBlk);
+  if (rc == SPARTA_OK) rc = rows_map(&m.do_block, a.dO, a.dtype, D, q_rows, kBlk);
+  if (rc == SPARTA_OK) rc = rows_map(&m.k_block, a.K, a.dtype, D, k_rows, kBlk);
+  if (rc == SPARTA_OK) rc = rows_map(&m.v_block, a.V, a.dtype, D, k_rows, kBlk);
+  if (rc != SPARTA_OK) return rc;
+  PassParams kv = {}, q = {};
+  kv.out1 = a.dK; kv.out2 = a.dV;
+  kv.by_head = kv_exceeds_l2(a.heads, a.Nt, D);
+  kv.split = w.kv.split; kv.split_steps = w.kv.split_steps;
+  kv.partial = reinterpret_cast<float*>(ws + w.partial_kv);
+  kv.tickets = reinterpret_cast<uint32_t*>(ws + w.tickets_kv);
+  q.out1 = a.dQ;
+  q.by_head = kv_exceeds_l2(a.kv_heads, a.Ns, D);
+  q.split = w.q.split; q.split_steps = w.q.split_steps;
+  q.partial = reinterpret_cast<float*>(ws + w.partial_q);
+  q.tickets = tickets_q;
+  const long long kv_ctas = a.dK ? (long long)a.kv_heads * w.kv.tiles * w.kv.split : 0;
+  const long long q_ctas = a.dQ ? (long long)a.heads * w.q.tiles * w.q.split : 0;
+  if (kv_ctas + q_ctas > 0x7fffffffll) return SPARTA_ERR_SHAPE;
+  auto launch = [&](auto kern, SmemAttrOnce& attr) {
+    constexpr int kSmem = BwdCfg<true, D>::kSmem > BwdCfg<false, D>::kSmem ? BwdCfg<true, D>::kSmem : BwdCfg<false, D>::kSmem;
+    if (cudaError_t e = attr.ensure(kern, kSmem); e != cudaSuccess) return static_cast<int>(e);
+    kern<<<static_cast<unsigned>(kv_ctas + q_ctas), BwdCfg<true, D>::kThreads, kSmem, st>>>(m, p, kv, q, static_cast<int>(kv_ctas));
+    return launch_status();
+  };
+  static SmemAttrOnce attr_whole, attr_split;
+  return w.kv.split > 1 || w.q.split > 1 ? launch(attn_bwd_kernel<D, FMT, MASK, DROP, true>, attr_split)
+                                         : launch(attn_bwd_kernel<D, FMT, MASK, DROP, false>, attr_whole);
 }
 
 template <int D, int FMT>
