@@ -57,7 +57,7 @@ struct Attn64Params {
 };
 
 template <int FMT, bool DROP>
-__global__ void __launch_bounds__(kThreads, kCtasPerSM)
+__global__ void __launch_bounds__(kThreads, DROP ? 3 : kCtasPerSM)
 attn_fwd_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, Attn64Params p) {
   using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
