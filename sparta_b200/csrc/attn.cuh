@@ -66,9 +66,6 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float v0, float v1) {
 // ---- words of 32 decisions about consecutive columns ----
 // In "split" order bit i is column 2 i and bit 16 + i column 2 i + 1: the two bits of a packed pair of 16-bit values are
 // 16 apart, so that one shift and one byte permutation make the mask of the pair.
-__device__ __forceinline__ uint32_t to_split32(uint32_t c) { return (c >> 1) | ((c & 1u) << 4); }        // column -> bit
-__device__ __forceinline__ uint32_t from_split32(uint32_t i) { return ((i & 15u) << 1) | (i >> 4); }  // bit -> column
-
 // 0xffff in each half whose bit (i, 16 + i) is set
 __device__ __forceinline__ uint32_t pair_mask(uint32_t word, int i) { return spread2(word << (15 - i)); }
 
@@ -109,26 +106,21 @@ __device__ __forceinline__ uint32_t mask_word32(const uint8_t* m) {
   return bits;
 }
 
-// the same in split order: the even bits gathered in the lower half, the odd ones in the upper
-__device__ __forceinline__ uint32_t mask_split32(const uint8_t* m) {
-  uint32_t x = mask_word32(m), t;
+// the even bits gathered in the lower half, the odd ones in the upper, and back
+__device__ __forceinline__ uint32_t split_bits32(uint32_t x) {
+  uint32_t t;
   t = (x ^ (x >> 1)) & 0x22222222u; x ^= t ^ (t << 1);
   t = (x ^ (x >> 2)) & 0x0c0c0c0cu; x ^= t ^ (t << 2);
   t = (x ^ (x >> 4)) & 0x00f000f0u; x ^= t ^ (t << 4);
   t = (x ^ (x >> 8)) & 0x0000ff00u; x ^= t ^ (t << 8);
   return x;
 }
-
-// 32 x 32 bits across a warp, lane l holding row l: afterwards lane l holds column l (bit i = bit l of row i).  Swaps
-// the off-diagonal halves of ever smaller squares.
-__device__ __forceinline__ uint32_t transpose_bits32(uint32_t x, int lane) {
-  uint32_t low = 0x0000ffffu;
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, s);
-    x = (lane & s) == 0 ? ((x & low) | ((y & low) << s)) : (((y >> s) & low) | (x & ~low));
-    low ^= low << (s >> 1);
-  }
+__device__ __forceinline__ uint32_t unsplit_bits32(uint32_t x) {
+  uint32_t t;
+  t = (x ^ (x >> 8)) & 0x0000ff00u; x ^= t ^ (t << 8);
+  t = (x ^ (x >> 4)) & 0x00f000f0u; x ^= t ^ (t << 4);
+  t = (x ^ (x >> 2)) & 0x0c0c0c0cu; x ^= t ^ (t << 2);
+  t = (x ^ (x >> 1)) & 0x22222222u; x ^= t ^ (t << 1);
   return x;
 }
 

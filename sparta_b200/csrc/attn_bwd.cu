@@ -33,9 +33,12 @@
 //   and keeps descriptors in uniform registers (335 -> 305 us for dK, dV of B4 H16 S4096 D64 before the other steps).
 //   warps 0 .. 15  scores and epilogue        warp 16  TMA producer        warp 17  MMA issue
 //
-// Masks and dropout are words of 32 decisions per row of the score matrix, even columns in the lower half.  In the
-// dK, dV pass a thread owns a key, so each lane makes the word of one query row over the warp's 32 keys and the warp
-// transposes the 32 x 32 bits.
+// The dK, dV pass needs the statistics of its columns, the query rows.  Read by threads that each own a row they were 16
+// vector loads of shared memory per warp and step, all lanes at one address, and took 45 % of its bandwidth; that pass
+// therefore reads and writes tensor memory in the fragment layout, where a thread has four rows and eight columns.
+//
+// Masks and dropout are words of 32 decisions per row of the score matrix (query): in the dQ pass each thread's own, in
+// the dK, dV pass each lane makes one and the threads fetch those of their eight columns from the lanes that made them.
 // The forward pass it belongs to: SparseAttention.forward (sparta/specializer/operators/sparse_attention.py:76-80),
 // whose gradients the reference takes through its three operators.
 #include <type_traits>
@@ -119,6 +122,24 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "=l"(reinterpret_cast<uint64_t&>(d))
       : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
   return d;
+}
+
+// Decisions about two columns (8 n + 2 (lane % 4) and the next) and the thread's four rows, as bytes: lane c of the warp
+// holds the word of column c, bit = row.
+struct ColumnMasks {
+  uint32_t c0, c1;
+};
+__device__ __forceinline__ ColumnMasks column_masks(uint32_t word, int n, int lane) {
+  const int c = 8 * n + 2 * (lane & 3);
+  const uint32_t w0 = __shfl_sync(0xffffffffu, word, c), w1 = __shfl_sync(0xffffffffu, word, c + 1);
+  return {((w0 >> (lane >> 2)) & 0x01010101u) * 0xffu, ((w1 >> (lane >> 2)) & 0x01010101u) * 0xffu};
+}
+__device__ __forceinline__ uint32_t packed_mask(const ColumnMasks& m, int r) {  // of a pair of 16-bit values in row r
+  return __byte_perm(m.c0, m.c1, r * 0x11 | (r + 4) * 0x1100);
+}
+__device__ __forceinline__ float2 mask_pair(float2 v, const ColumnMasks& m, int r) {
+  return make_float2(__uint_as_float(__float_as_uint(v.x) & __byte_perm(m.c0, 0, r * 0x1111)),
+                     __uint_as_float(__float_as_uint(v.y) & __byte_perm(m.c1, 0, r * 0x1111)));
 }
 
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -493,21 +514,21 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
       const bool mine = (e >> half) & 1;               // it is kept for this warp's rows
       const int blk = e >> 2;
       const uint32_t s_addr = s_base + (j % kSBuf) * C::kCols;
-      // words of decisions over this thread's 32 columns: made for a row of the score matrix, turned round where the
-      // thread is a key
+      // words of decisions over the warp's 32 x 32 scores, made for rows of the score matrix: for this thread's own over
+      // its columns (split order), or for query `lane` of the block over the warp's keys
       uint32_t mask_w = 0xffffffffu, keep_w = 0xffffffffu;
       if ((MASK || DROP) && mine) {
-        const int q_row = DKV ? blk * kBlk + (quarter & 1) * 32 + from_split32(lane) : grow;
+        const int q_row = DKV ? blk * kBlk + (quarter & 1) * 32 + lane : grow;
         const int word = DKV ? tile * (kTileM / 32) + quad : blk * (kBlk / 32) + (quarter & 1);
         if constexpr (MASK) {
-          mask_w = mask_split32(p.mask + (long long)q_row * p.Ns + word * 32);
-          if constexpr (DKV) mask_w = __shfl_sync(0xffffffffu, transpose_bits32(mask_w, lane), to_split32(lane));
+          mask_w = mask_word32(p.mask + (long long)q_row * p.Ns + word * 32);
+          if constexpr (!DKV) mask_w = split_bits32(mask_w);
         }
         if constexpr (DROP) {
           const int q_head = DKV ? head * p.group + h : head;
           if constexpr (DKV) key_row = philox_row(key, q_row, q_head);
           keep_w = philox_split32(key, key_row, t2, word, q_head);
-          if constexpr (DKV) keep_w = __shfl_sync(0xffffffffu, transpose_bits32(keep_w, lane), to_split32(lane));
+          if constexpr (DKV) keep_w = unsplit_bits32(keep_w);
         }
       }
       if (++k == pairs) { k = 0; ++h; }
@@ -516,35 +537,47 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
       if (!ok) continue;
       tc_fence_after_sync();
       // ---- P = exp2(scale log2(e) S - lse log2(e)) ----
-      const float4* nl4 = reinterpret_cast<const float4*>(stat_s + st * C::kStatFloats + quarter * 32);
+      const float* stat = stat_s + st * C::kStatFloats + quarter * 32 + 2 * (lane & 3);  // of this thread's columns
       float2 prob[16];
       uint32_t packed[16];
       if (mine) {
         uint32_t s[32];
-        tmem_ld_x32(s_addr, s);
+        if constexpr (DKV) {
+          tmem_ld_16x256b_x4(s_addr, s);
+          tmem_ld_16x256b_x4(s_addr + (16u << 16), s + 16);
+        } else {
+          tmem_ld_x32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(s));
+        }
         tmem_ld_wait();
+        auto exp_pair = [&](int i, float2 n) {  // scores 2 i, 2 i + 1
+          const float2 v = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, n);
+          return make_float2(ex2_approx(v.x), ex2_approx(v.y));
+        };
+        if constexpr (DKV) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          float2 n0 = nl, n1 = nl;
-          if constexpr (DKV) {
-            const float4 n = nl4[i / 2];
-            n0 = make_float2(n.x, n.y);
-            n1 = make_float2(n.z, n.w);
+          for (int n = 0; n < 4; ++n) {
+            const float2 stats = *reinterpret_cast<const float2*>(stat + 8 * n);
+            const ColumnMasks m = MASK ? column_masks(mask_w, n, lane) : ColumnMasks{};
+            const ColumnMasks d = DROP ? column_masks(keep_w, n, lane) : ColumnMasks{};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {  // rows lane / 4 + 8 r
+              const int i = (r >> 1) * 8 + 2 * n + (r & 1);
+              float2 v = exp_pair(i, stats);
+              if constexpr (MASK) v = mask_pair(v, m, r);
+              prob[i] = v;
+              packed[i] = pack2<T>(v.x, v.y);
+              if constexpr (DROP) packed[i] &= packed_mask(d, r);
+            }
           }
+        } else {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float2 v = fma2(make_float2(__uint_as_float(s[2 * (i + q)]), __uint_as_float(s[2 * (i + q) + 1])), scale2, q ? n1 : n0);
-            v.x = ex2_approx(v.x);
-            v.y = ex2_approx(v.y);
+          for (int i = 0; i < 16; ++i) {
+            float2 v = exp_pair(i, nl);
             if constexpr (MASK) {
-              v.x = (mask_w >> (i + q)) & 1u ? v.x : 0.f;
-              v.y = (mask_w >> (i + q + 16)) & 1u ? v.y : 0.f;
+              v.x = (mask_w >> i) & 1u ? v.x : 0.f;
+              v.y = (mask_w >> (i + 16)) & 1u ? v.y : 0.f;
             }
-            prob[i + q] = v;
-            if constexpr (DKV) {
-              packed[i + q] = pack2<T>(v.x, v.y);
-              if constexpr (DROP) packed[i + q] &= pair_mask(keep_w, i + q);
-            }
+            prob[i] = v;
           }
         }
       } else {
@@ -552,8 +585,9 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
         for (int i = 0; i < 16; ++i) packed[i] = 0;
       }
       if constexpr (DKV) {
-        if (there) {
-          tmem_st_x16(s_addr, packed);  // over columns that this thread has read
+        if (there) {  // over columns that this warp has read
+          tmem_st_16x128b_x4(s_addr, packed);
+          tmem_st_16x128b_x4(s_addr + (16u << 16), packed + 8);
           tmem_st_wait();
         }
       }
@@ -563,31 +597,45 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
       // ---- dS = P (dP - delta) ----
       if (!mbar_wait_warp(dp_full, j & 1)) { ok = false; continue; }
       tc_fence_after_sync();
-      const float4* nd4 = nl4 + C::kCols / 4;
       if (mine) {
         uint32_t s[32];
-        tmem_ld_x32(dp_addr, s);
+        if constexpr (DKV) {
+          tmem_ld_16x256b_x4(dp_addr, s);
+          tmem_ld_16x256b_x4(dp_addr + (16u << 16), s + 16);
+        } else {
+          tmem_ld_x32(dp_addr, *reinterpret_cast<uint32_t(*)[32]>(s));
+        }
         tmem_ld_wait();
+        const float2 up2 = make_float2(up, up);
+        if constexpr (DKV) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          float2 n0 = nd, n1 = nd;
-          if constexpr (DKV) {
-            const float4 n = nd4[i / 2];
-            n0 = make_float2(n.x, n.y);
-            n1 = make_float2(n.z, n.w);
-          }
+          for (int n = 0; n < 4; ++n) {
+            const float2 stats = *reinterpret_cast<const float2*>(stat + C::kCols + 8 * n);
+            const ColumnMasks m = MASK ? column_masks(mask_w, n, lane) : ColumnMasks{};
+            const ColumnMasks d = DROP ? column_masks(keep_w, n, lane) : ColumnMasks{};
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float2 v = make_float2(__uint_as_float(s[2 * (i + q)]), __uint_as_float(s[2 * (i + q) + 1]));
-            if constexpr (DROP) {
-              v = mul2(v, make_float2(up, up));
-              v.x = (keep_w >> (i + q)) & 1u ? v.x : 0.f;
-              v.y = (keep_w >> (i + q + 16)) & 1u ? v.y : 0.f;
+            for (int r = 0; r < 4; ++r) {
+              const int i = (r >> 1) * 8 + 2 * n + (r & 1);
+              float2 v = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+              if constexpr (DROP) v = mask_pair(mul2(v, up2), d, r);
+              v = mul2(prob[i], add2(v, stats));
+              packed[i] = pack2<T>(v.x, v.y);
+              // a masked score's probability is zero, and so is its dS whatever stands in V
+              if constexpr (MASK) packed[i] &= packed_mask(m, r);
             }
-            v = mul2(prob[i + q], add2(v, q ? n1 : n0));
-            packed[i + q] = pack2<T>(v.x, v.y);
-            // a masked score's probability is zero, and so is its dS whatever stands in V
-            if constexpr (MASK) packed[i + q] &= pair_mask(mask_w, i + q);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 v = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+            if constexpr (DROP) {
+              v = mul2(v, up2);
+              v.x = (keep_w >> i) & 1u ? v.x : 0.f;
+              v.y = (keep_w >> (i + 16)) & 1u ? v.y : 0.f;
+            }
+            v = mul2(prob[i], add2(v, nd));
+            packed[i] = pack2<T>(v.x, v.y);
+            if constexpr (MASK) packed[i] &= pair_mask(mask_w, i);
           }
         }
       } else {
@@ -595,7 +643,12 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
         for (int i = 0; i < 16; ++i) packed[i] = 0;
       }
       if (there) {
-        tmem_st_x16(dp_addr, packed);
+        if constexpr (DKV) {
+          tmem_st_16x128b_x4(dp_addr, packed);
+          tmem_st_16x128b_x4(dp_addr + (16u << 16), packed + 8);
+        } else {
+          tmem_st_x16(dp_addr, packed);
+        }
         tmem_st_wait();
       }
       tc_fence_before_sync();
