@@ -124,22 +124,26 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
-// Decisions about two columns (8 n + 2 (lane % 4) and the next) and the thread's four rows, as bytes: lane c of the warp
-// holds the word of column c, bit = row.
+// Decisions about two columns (8 n + 2 (lane % 4) and the next) and the thread's four rows (lane / 4 + 8 r), at the top
+// of byte r; lane c of the warp holds the word of column c, bit = row.  A byte permutation spreads the tops into masks.
 struct ColumnMasks {
   uint32_t c0, c1;
 };
 __device__ __forceinline__ ColumnMasks column_masks(uint32_t word, int n, int lane) {
-  const int c = 8 * n + 2 * (lane & 3);
-  const uint32_t w0 = __shfl_sync(0xffffffffu, word, c), w1 = __shfl_sync(0xffffffffu, word, c + 1);
-  return {((w0 >> (lane >> 2)) & 0x01010101u) * 0xffu, ((w1 >> (lane >> 2)) & 0x01010101u) * 0xffu};
+  const int c = 8 * n + 2 * (lane & 3), up = 7 - (lane >> 2);
+  return {__shfl_sync(0xffffffffu, word, c) << up, __shfl_sync(0xffffffffu, word, c + 1) << up};
+}
+__device__ __forceinline__ uint32_t permute_signs(uint32_t a, uint32_t b, uint32_t selector) {  // selector nibbles 8 + byte: its sign
+  uint32_t m;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(m) : "r"(a), "r"(b), "r"(selector));
+  return m;
 }
 __device__ __forceinline__ uint32_t packed_mask(const ColumnMasks& m, int r) {  // of a pair of 16-bit values in row r
-  return __byte_perm(m.c0, m.c1, r * 0x11 | (r + 4) * 0x1100);
+  return permute_signs(m.c0, m.c1, 0xcc88u + r * 0x1111u);
 }
 __device__ __forceinline__ float2 mask_pair(float2 v, const ColumnMasks& m, int r) {
-  return make_float2(__uint_as_float(__float_as_uint(v.x) & __byte_perm(m.c0, 0, r * 0x1111)),
-                     __uint_as_float(__float_as_uint(v.y) & __byte_perm(m.c1, 0, r * 0x1111)));
+  return make_float2(__uint_as_float(__float_as_uint(v.x) & permute_signs(m.c0, 0, 0x8888u + r * 0x1111u)),
+                     __uint_as_float(__float_as_uint(v.y) & permute_signs(m.c1, 0, 0x8888u + r * 0x1111u)));
 }
 
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
