@@ -65,11 +65,11 @@ def _compile(src: str, force: bool, verbose: bool) -> str:
 
 
 def _compile_torch_ops(force: bool, verbose: bool) -> str:
-    from torch.utils import cpp_extension
     obj, path = os.path.join(OBJ_DIR, 'torch_ops.o'), os.path.join(CSRC, 'torch_ops.cpp')
     header = os.path.join(ROOT, 'include', 'sparta_b200.h')
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(path), os.path.getmtime(header)):
         return obj
+    from torch.utils import cpp_extension
     includes = [*cpp_extension.include_paths('cuda'), sysconfig.get_paths()['include']]
     cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-DTORCH_EXTENSION_NAME=_torch_ops', '-DTORCH_API_INCLUDE_EXTENSION_H',
            *[f'-isystem{d}' for d in includes], '-c', path, '-o', obj]
@@ -82,9 +82,9 @@ def _compile_torch_ops(force: bool, verbose: bool) -> str:
 
 
 def _link_torch_ops(obj: str, force: bool):
-    from torch.utils import cpp_extension
     if not force and os.path.exists(TORCH_OPS_PATH) and os.path.getmtime(TORCH_OPS_PATH) >= os.path.getmtime(obj):
         return
+    from torch.utils import cpp_extension
     dirs = cpp_extension.library_paths('cuda')
     cmd = ['g++', '-shared', '-o', TORCH_OPS_PATH, obj, *[f'-L{d}' for d in (LIB_DIR, *dirs)], '-lsparta_b200', '-lc10', '-lc10_cuda',
            '-ltorch_cpu', '-ltorch_cuda', '-ltorch', '-ltorch_python', '-Wl,-rpath,$ORIGIN', f'-Wl,-rpath,{dirs[0]}']
