@@ -48,8 +48,8 @@ class SparseAttention(OperatorBase):
 
     ``forward(query, key, value, rng=None, positions=None, key_positions=None)``: ``rng`` replaces the module's own
     random numbers (see ``SparseDropout``), the positions go to ``rotary``.  Inputs are finite: a NaN or an infinity
-    in a key or value row reaches every query row that shares a kept 64 x 64 block, or its neighbour in the same pair
-    of block rows, with it.
+    in a row reaches, forward and backward, all rows that share a kept 64 x 64 block with it, masked elements of the block
+    included, and those of that block's neighbour in the same 128 rows.
 
     Shape: Q :math:`(B \times H, N_{target}, E)`; K, V :math:`(B \times H, N_{source}, E)`, or with fewer heads, each
     shared by as many consecutive heads of Q; any leading dimensions; output like Q.

@@ -422,3 +422,79 @@ def test_offsets_beyond_32_bits():
     grads1 = torch.autograd.grad(out1, small, do[-3:])
     for a, b in zip((out,) + grads, (out1,) + grads1):
         assert torch.equal(a[-3:], b)
+
+
+def test_nan_reaches_the_gradients():
+    """A NaN in one query row makes that row's output and dQ, and the dK, dV of the keys it sees, NaN: none turns into a
+    number.  Blocks of other pairs of block rows and columns do not see it."""
+    q, k, v, do = inputs(torch.bfloat16, 1, 1, 256, 256, 64)
+    q[0, 7, 3] = float('nan')
+    mask = torch.zeros((256, 256), dtype=torch.uint8)
+    for i in range(0, 256, 64):
+        mask[i:i + 64, i:i + 64] = 1
+    out, dq, dk, dv = step(build(mask, q, k, v), q, k, v, do)
+    for x in (out, dq):
+        assert bool(torch.isnan(x[0, 7]).all()) and bool(torch.isfinite(x[0, 8:]).all())
+    for x in (dk, dv):
+        assert bool(torch.isnan(x[0, :64]).all()) and bool(torch.isfinite(x[0, 128:]).all())
+
+
+def test_two_graphs_replayed_in_turn():
+    """Two captured steps of one operator keep apart: neither's buffers are the other's."""
+    q, k, v, do = inputs(torch.float16, 2, 2, 256, 256, 64)
+    op = build(block_mask(256, 256, 0.6), q, k, v, dropout=0.2)
+    op.check_status = False
+    eager = [t.cuda().requires_grad_() for t in (q, k, v)]
+    alive = op(*eager, rng=rng(0, 0))  # an eager graph of its own that lives on
+    cases = []
+    for seed in (1, 2):
+        leaves = [t.cuda().requires_grad_() for t in inputs(torch.float16, 2, 2, 256, 256, 64, seed=seed)[:3]]
+        d, numbers = do.cuda(), rng(seed, 5)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(op(*leaves, rng=numbers), leaves, d)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = op(*leaves, rng=numbers)
+            held = (out,) + torch.autograd.grad(out, leaves, d)
+        want = step(op, *(t.detach().cpu() for t in leaves), do, rng=rng(seed, 5))
+        cases.append((graph, held, want, leaves, d, numbers))
+    for _ in range(2):
+        for graph, *_ in cases:
+            graph.replay()
+    torch.cuda.synchronize()
+    for _, held, want, *_ in cases:
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(alive, eager, do.cuda()))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_half_precision_on_the_three_operators(dtype):
+    """fused=False, built through sparta.nn.build: dropout and shared heads, at the repository's bar for half types."""
+    import sparta_b200
+    q, k, v, do = inputs(dtype, 4, 2, 128, 192, 64)
+    mask = block_mask(128, 192, 0.7, elements=True)
+    op = SparseAttention(mask.cuda(), fused=False, dropout=0.25)
+    sparta_b200.nn.build(op, [q.cuda(), k.cuda(), v.cuda()], {'root': config()})
+    keep = oracle.dropout_keep(3, 9, 4, 128, 192, 0.25)
+    got = step(op, q, k, v, do, rng=rng(3, 9))
+    want = oracle.attention(q, k, v, do, mask, 0.125, keep, oracle.dropout_scale(0.25))
+    for x, y in zip(got, want):
+        scale = max(1.0, y.abs().max().item())  # the scores' gradients pass through the type three times
+        torch.testing.assert_close(x.detach().double().cpu() / scale, y / scale, atol=2e-2, rtol=2e-2)
+    fused = build(mask, q, k, v, dropout=0.25)
+    out = step(fused, q, k, v, do, rng=rng(3, 9))[0]
+    torch.testing.assert_close(out, got[0], atol=2e-2, rtol=2e-2)
+
+
+def test_random_state_travels_with_the_module():
+    q, k, v, do = inputs(torch.float16, 2, 2, 128, 128, 64)
+    mask = block_mask(128, 128, 1.0)
+    a, b = (build(mask, q, k, v, dropout=0.5) for _ in range(2))
+    a(q.cuda(), k.cuda(), v.cuda())
+    b.load_state_dict(a.state_dict())
+    assert torch.equal(a(q.cuda(), k.cuda(), v.cuda()), b(q.cuda(), k.cuda(), v.cuda()))
+    a.eval(), b.eval()
+    assert torch.equal(a(q.cuda(), k.cuda(), v.cuda()), build(mask, q, k, v)(q.cuda(), k.cuda(), v.cuda()))
