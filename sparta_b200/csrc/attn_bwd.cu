@@ -7,9 +7,8 @@
 //   dS = P (dP - delta)      dQ = scale dS K       dK = scale dS^T Q        (K, V shared by heads: summed over them)
 //
 // Two passes over the kept blocks, each with its sums in tensor memory from the first block to the last, so that every
-// gradient is written once, in a fixed order of additions: one pass
-// owns 128 query rows and walks the kept key blocks (dQ), the other owns 128 key rows and walks the query blocks of
-// every head that shares them (dK, dV).  That is seven products per kept block instead of the five of a single pass,
+// gradient is written once, in a fixed order of additions: one pass owns 128 query rows and walks the kept key blocks
+// (dQ), the other owns 128 key rows and walks the query blocks of every head that shares them (dK, dV).  That is seven products per kept block instead of the five of a single pass,
 // which would have to add 128 x D 32-bit partial sums of dQ per block to global memory (in an order that changes from
 // run to run): 32 to 64 KB of atomic traffic per 128 x 128 scores, more than L2 takes at the rate of the products.
 //
@@ -21,17 +20,21 @@
 // P' and dS go back into tensor memory, over the columns that their own thread has just read, as the A operand of the
 // last products; B1 and B2 serve twice, K-major for S and dP, MN-major (the head dim contiguous) for the sums.
 //
-// Schedule.  A step is a pair of blocks, 128 columns of scores for 128 rows, in two phases: P from S, then dS from P and
-// dP; sixteen warps, four threads per row with 32 columns each.  One warp issues every MMA: when P of step j is in
-// place, P'^T dO of j and then S of a later step; when dS of j is in place, dS B1 of j and then dP of the next step.
-// MMAs of one thread execute in order, so S of a later step may take the columns that P' is being read from, and the
-// tensor pipe works on one half of a step while the threads work on the other.  Tensor memory: S 128 columns (twice for
-// head dim 64, so that the next S is never waited for), dP 128, the sums D each.
-//   Steps of one block (N = 64 instead of 128) make an MMA read 6 KB of shared memory for 32 cycles of math and double
-//   the number of MMAs, which one warp issues at one per 60 to 80 cycles: 1.6 times the time for head dim 128.
+// Schedule.  A step is 128 columns of scores (two blocks) for head dim 128, 64 (one) for head dim 64, for 128 rows, in
+// two phases: P from S, then dS from P and dP; one warp for every 32 rows x 32 columns.  Another warp issues every MMA:
+// when P of step j is in place, P'^T dO of j and then S of a later step; when dS of j is in place, dS B1 of j and then
+// dP of the next step.  MMAs of one thread execute in order, so S of a later step may take the columns that P' is being
+// read from, and the tensor pipe works on one half of a step while the threads work on the other.
+//   Head dim 128: tensor memory is full with S, dP (128 columns each) and the sums; one CTA of 18 warps per SM.  With
+//   steps of one block an MMA reads 6 KB of shared memory for 32 cycles of math, and there are twice as many to issue at
+//   one per 60 to 80 cycles: 1.4 times the time (H16 S8192 on 4 key heads, both passes: 1012 us against 705).
+//   Head dim 64: half the tensor memory per CTA (S twice in the dQ pass), so that two CTAs of 10 warps share an SM and
+//   one computes while the other waits or starts up: steps of two blocks with one CTA measured 595 us against 490 us
+//   (B4 H16 S4096, both passes).
 //   The warp number and what MMAs are addressed with go through a shuffle: the compiler then knows them to be uniform
-//   and keeps descriptors in uniform registers (335 -> 305 us for dK, dV of B4 H16 S4096 D64 before the other steps).
-//   warps 0 .. 15  scores and epilogue        warp 16  TMA producer        warp 17  MMA issue
+//   and keeps descriptors in uniform registers (dK, dV of B4 H16 S4096 D64 335 -> 305 us before the other steps).
+// What bounds it now: the chain of a step -- scores, exponentials, hand-over, products -- of the tiles in flight; no
+// unit is busy more than half of the time (see the profile of the kernel).
 //
 // The dK, dV pass needs the statistics of its columns, the query rows.  Read by threads that each own a row they were 16
 // vector loads of shared memory per warp and step, all lanes at one address, and took 45 % of its bandwidth; that pass
@@ -52,15 +55,13 @@ namespace {
 
 using namespace tc;
 
-constexpr int kBlk = 64;        // mask block edge = rows of B1, B2 per step
+constexpr int kBlk = 64;        // mask block edge
 constexpr int kTileM = 128;     // rows of A1, A2 per CTA (two blocks)
 constexpr int kMaxBlocks = 1024;  // blocks along the streamed side (65536 rows)
 
 struct BwdParams {
-  const int32_t* row_ptr;
-  const int32_t* idx;
   const uint8_t* mask;      // [Nt, Ns] or null
-  const uint8_t* present;   // [Nt / 64, present_pitch]: block kept (built by the first kernel)
+  const uint8_t* present;   // [Nt / 64, present_pitch]: block kept (made by the first kernel)
   const float* neg_lse;     // [heads, Nt]: -lse * log2(e), -inf for a row without any score
   const float* neg_delta;   // [heads, Nt]
   int Nt, Ns, heads, kv_heads, group;
@@ -221,11 +222,12 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
   uint8_t* a2_s = a1_s + C::kABytes;
   uint8_t* b1_s = a2_s + C::kABytes;                        // [kStages]
   uint8_t* b2_s = b1_s + kStages * C::kBBytes;              // [kStages]
-  float* stat_s = reinterpret_cast<float*>(b2_s + kStages * C::kBBytes);  // [kStages][neg_lse 128, neg_delta 128]
+  float* stat_s = reinterpret_cast<float*>(b2_s + kStages * C::kBBytes);  // [kStages][neg_lse, neg_delta of the step's columns]
   uint16_t* ulist = reinterpret_cast<uint16_t*>(stat_s + kStages * C::kStatFloats);  // (block << 2) | presence bits
   uint8_t* kmask = reinterpret_cast<uint8_t*>(ulist + kMaxBlocks);
-  uint64_t* a_full = reinterpret_cast<uint64_t*>(kmask + kMaxBlocks);
-  uint64_t* full1 = a_full + 1;         // [kStages] B1 (and the statistics) of a step have landed
+  uint64_t* a1_full = reinterpret_cast<uint64_t*>(kmask + kMaxBlocks);
+  uint64_t* a2_full = a1_full + 1;
+  uint64_t* full1 = a2_full + 1;        // [kStages] B1 (and the statistics) of a step have landed
   uint64_t* empty1 = full1 + kStages;   // [kStages] the MMAs that read it are done
   uint64_t* full2 = empty1 + kStages;   // [kStages] B2 likewise
   uint64_t* empty2 = full2 + kStages;
@@ -263,7 +265,8 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
 
   // ------------------------------ prologue ------------------------------
   if (threadIdx.x == 0) {
-    mbar_init(a_full, 1);
+    mbar_init(a1_full, 1);
+    mbar_init(a2_full, 1);
     for (int st = 0; st < kStages; ++st) {
       mbar_init(&full1[st], 1);
       mbar_init(&empty1[st], 1);
@@ -289,16 +292,10 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
       kmask[r] = static_cast<uint8_t>((two & 1u) | ((two >> 7) & 2u));
     }
   } else {
-    for (int k = threadIdx.x; k < nbc; k += kThreads) kmask[k] = 0;
-    __syncthreads();
-    // the two block rows are consecutive in the BCSR array: entry = (block row << 16) | key block
-    const int e1 = __ldg(p.row_ptr + min(blk0 + 2, nbr));
-    for (int e = __ldg(p.row_ptr + blk0) + threadIdx.x; e < e1; e += kThreads) {
-      const int v = __ldg(p.idx + e);
-      const int kb = v & 0xffff, r = static_cast<int>(static_cast<uint32_t>(v) >> 16) - blk0;
-      if (kb < nbc && r >= 0 && r < 2)
-        atomicOr(reinterpret_cast<unsigned int*>(kmask + (kb & ~3)), (1u << r) << (8 * (kb & 3)));
-    }
+    const uint8_t* row0 = p.present + (long long)blk0 * p.present_pitch;
+    const bool second = blk0 + 1 < nbr;                // the last tile may be one block row high
+    for (int k = threadIdx.x; k < nbc; k += kThreads)
+      kmask[k] = static_cast<uint8_t>(__ldg(row0 + k) | (second ? __ldg(row0 + p.present_pitch + k) << 1 : 0));
   }
   __syncthreads();
   if (warp == 0) {  // ordered compaction of the merged list
@@ -340,11 +337,11 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
   if (warp == kWarpLoad) {
     // ------------------------------ producer ------------------------------
     if (lane == 0 && steps > 0) {
-      mbar_arrive_expect_tx(a_full, 2 * C::kABytes);
-      for (int c = 0; c < kChunks; ++c) {
-        tma_load_2d(a1_s + c * (kTileM * 128), &tm_a1, c * 64, (int)a_row0, a_full);
-        tma_load_2d(a2_s + c * (kTileM * 128), &tm_a2, c * 64, (int)a_row0, a_full);
-      }
+      auto resident = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar) {
+        mbar_arrive_expect_tx(bar, C::kABytes);
+        for (int c = 0; c < kChunks; ++c) tma_load_2d(dst + c * (kTileM * 128), map, c * 64, (int)a_row0, bar);
+      };
+      resident(a1_s, &tm_a1, a1_full);  // with the first B1: the first S needs nothing else
       bool ok = true;
       int h = h0, k = k0;
       for (int j = 0; j < steps; ++j) {
@@ -362,6 +359,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
             bulk_load(stat_s + st * C::kStatFloats + C::kCols + b * kBlk, p.neg_delta + row, kBlk * 4, &full1[st]);
           }
         }
+        if (j == 0) resident(a2_s, &tm_a2, a2_full);
         if (!mbar_wait(&empty2[st], par)) { ok = false; break; }
         mbar_arrive_expect_tx(&full2[st], nblk * kBlk * D * 2);
         for (int b = 0; b < nblk; ++b) {
@@ -405,7 +403,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
     };
     // the last pair of the list may be a single block
     auto blocks_of = [&](int j) { return C::kBlocks == 2 && !((count & 1) && (step0 + j + 1) % pairs == 0) ? 2 : 1; };
-    bool ok = steps == 0 || mbar_wait_warp(a_full, 0);
+    bool ok = steps == 0 || mbar_wait_warp(a1_full, 0);
 #pragma unroll
     for (int j = 0; j < kSBuf; ++j) {  // the first scores
       if (j >= steps || !ok) break;
@@ -419,7 +417,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
       __syncwarp();
     }
     if (ok && steps > 0) {
-      ok = mbar_wait_warp(&full2[0], 0);
+      ok = mbar_wait_warp(a2_full, 0) && mbar_wait_warp(&full2[0], 0);
       if (ok) {
         tc_fence_after_sync();
         if (elect_one()) {
@@ -889,7 +887,7 @@ size_t attn_bwd_workspace(int heads, int kv_heads, int Nt, int Ns, int D, long l
 int attn_bwd_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* status, cudaStream_t st) {
   if (a.Ns / kBlk > kMaxBlocks || a.Nt / kBlk > kMaxBlocks) return SPARTA_ERR_UNSUPPORTED;
   BwdParams p = {};
-  p.row_ptr = a.row_ptr; p.idx = a.idx; p.mask = a.mask;
+  p.mask = a.mask;
   p.Nt = a.Nt; p.Ns = a.Ns; p.heads = a.heads; p.kv_heads = a.kv_heads; p.group = a.heads / a.kv_heads;
   p.scale = a.scale; p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = status;
