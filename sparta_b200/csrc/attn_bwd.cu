@@ -595,7 +595,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[j % kSBuf]);
+      mbar_arrive_if(&p_full[j % kSBuf], lane == 0);
       // ---- dS = P (dP - delta) ----
       if (!mbar_wait_warp(dp_full, j & 1)) { ok = false; continue; }
       tc_fence_after_sync();
@@ -655,7 +655,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      mbar_arrive_if(ds_full, lane == 0);
     }
     // ---- epilogue: the sums -> global, one row per thread, 32-column pieces dealt to the threads of a row ----
     if (ok && steps > 0 && !mbar_wait_warp(done, 0)) ok = false;
