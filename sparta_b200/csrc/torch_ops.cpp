@@ -261,7 +261,7 @@ sparta_attn_train_args attention_args(const Tensor& q, const Tensor& k, const Te
   a.K = k.const_data_ptr();
   a.V = v.const_data_ptr();
   a.O = out.data_ptr();
-  a.lse = lse.data_ptr<float>();
+  a.lse = lse.defined() ? lse.data_ptr<float>() : nullptr;
   a.row_ptr = row_ptr.const_data_ptr<int32_t>();
   a.bcsr_idx = bcsr.const_data_ptr<int32_t>();
   a.mask = mask ? mask->const_data_ptr<uint8_t>() : nullptr;
@@ -286,6 +286,15 @@ void check_words(const Tensor& status, const AttentionCall& c) {
     TORCH_CHECK(!status.any().item<bool>(), "fused sparse attention: a bounded wait ran out on the device; the output is invalid");
 }
 
+void run_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse, const Tensor& row_ptr,
+                   const Tensor& bcsr, const OptTensor& mask, const Tensor& status, const OptTensor& rng, const AttentionCall& c) {
+  if (out.numel() == 0) return;
+  const c10::cuda::CUDAGuard guard(q.device());
+  const sparta_attn_train_args a = attention_args(q, k, v, out, lse, row_ptr, bcsr, mask, status, rng, c);
+  check_status(sparta_attn_train_fwd(&a, stream_of(q)), "sparta_attn_train_fwd");
+  check_words(status, c);
+}
+
 struct AttentionFn : torch::autograd::Function<AttentionFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& row_ptr,
                         const Tensor& bcsr, const OptTensor& mask, const Tensor& status, const OptTensor& rng, double p, double scale,
@@ -294,12 +303,7 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     const Tensor q = attention_rows(query, c.Nt), k = attention_rows(key, c.Ns), v = attention_rows(value, c.Ns);
     Tensor out = at::empty(query.sizes(), query.options());
     Tensor lse = at::empty({q.size(0), c.Nt}, query.options().dtype(at::kFloat));
-    if (out.numel() > 0) {
-      const c10::cuda::CUDAGuard guard(q.device());
-      const sparta_attn_train_args a = attention_args(q, k, v, out, lse, row_ptr, bcsr, mask, status, rng, c);
-      check_status(sparta_attn_train_fwd(&a, stream_of(q)), "sparta_attn_train_fwd");
-      check_words(status, c);
-    }
+    run_attention(q, k, v, out, lse, row_ptr, bcsr, mask, status, rng, c);
     // an element mask and the random numbers are read again: autograd refuses if they were rewritten in place since
     ctx->save_for_backward({q, k, v, out, lse, row_ptr, bcsr, tensor_of(mask), status, tensor_of(rng)});
     ctx->saved_data["p"] = p;
@@ -355,15 +359,33 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
   }
 };
 
+void check_attention(const Tensor& x, const Tensor& query, int64_t n, int64_t dim, const char* name) {
+  check_cuda(x);
+  TORCH_CHECK_VALUE(x.dim() >= 2 && x.size(-2) == n && x.size(-1) == dim, "expect ", name, " shape (?, ", n, ", ", dim, "), got ",
+                    x.sizes());
+  TORCH_CHECK_TYPE(x.scalar_type() == query.scalar_type() && x.device() == query.device(),
+                   "query, key and value have to be of one type on one device");
+}
+
 Tensor attention(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& row_ptr, const Tensor& bcsr,
                  const OptTensor& mask, const Tensor& status, const OptTensor& rng, double p, double scale, int64_t seed, int64_t call,
-                 int64_t nnz, int64_t Nt, int64_t Ns, bool check) {
-  check_cuda(query);
-  check_cuda(key);
-  check_cuda(value);
+                 int64_t nnz, int64_t Nt, int64_t Ns, int64_t dim, bool check) {
+  check_attention(query, query, Nt, dim, "query");
+  check_attention(key, query, Ns, dim, "key");
+  check_attention(value, query, Ns, dim, "value");
+  const int64_t q_heads = query.numel() / (Nt * dim), k_heads = key.numel() / (Ns * dim), v_heads = value.numel() / (Ns * dim);
+  TORCH_CHECK_VALUE(k_heads == v_heads && k_heads > 0 && q_heads % k_heads == 0, q_heads, " query heads cannot share ", k_heads,
+                    " key and ", v_heads, " value heads");
+  TORCH_CHECK_VALUE(q_heads <= INT_MAX && Nt <= INT_MAX && Ns <= INT_MAX, "attention: a dimension beyond 31 bits");
   rng_pointer(rng, query);
-  return AttentionFn::apply(query, key, value, row_ptr, bcsr, mask, status, rng, p, scale,
-                            std::vector<int64_t>{seed, call, nnz, Nt, Ns, check});
+  if (at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad()))
+    return AttentionFn::apply(query, key, value, row_ptr, bcsr, mask, status, rng, p, scale,
+                              std::vector<int64_t>{seed, call, nnz, Nt, Ns, check});
+  const at::NoGradGuard no_grad;  // nothing to differentiate: no row sums are kept
+  const Tensor out = at::empty(query.sizes(), query.options());
+  run_attention(attention_rows(query, Nt), attention_rows(key, Ns), attention_rows(value, Ns), out, Tensor(), row_ptr, bcsr, mask,
+                status, rng, {p, scale, seed, call, nnz, Nt, Ns, check});
+  return out;
 }
 
 }  // namespace

@@ -91,13 +91,10 @@ class SparseAttention(OperatorBase):
             _lib.require_cuda(query)
             p, numbers = self._dropout.p, self._dropout._counter.next(rng)
         if self.ready and self._use_fused and (self._fused_request is True or query.dtype in FUSED_DTYPES):
-            group = self._check_heads(query, key, value)
-            wants_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, value))
-            if not wants_grad and p == 0.0 and group == 1:
-                return self._fused_forward(query.detach(), key.detach(), value.detach())
             # the fused backward pass lists the blocks along both sides
-            if not wants_grad or self._fused_request is True or self._Nt // FUSED_BLOCK <= FUSED_MAX_BLOCKS:
-                return self._fused_train(query, key, value, p, numbers)
+            if (self._Nt // FUSED_BLOCK <= FUSED_MAX_BLOCKS or self._fused_request is True
+                    or not (torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, value)))):
+                return self._fused(query, key, value, p, numbers)
         shape = query.shape
         if query.dim() != 3 or key.shape[:-2] != query.shape[:-2]:
             query, key, value = self._flat_heads(query, key, value)
@@ -129,13 +126,14 @@ class SparseAttention(OperatorBase):
             key, value = key.repeat_interleave(group, 0), value.repeat_interleave(group, 0)
         return query, key, value
 
-    def _fused_train(self, query, key, value, p: float, numbers: DropoutKey) -> torch.Tensor:
+    def _fused(self, query, key, value, p: float, numbers: DropoutKey) -> torch.Tensor:
         idx = self._sparse_port.indexes
         if self._attn_status is None or self._attn_status.device != query.device:
             self._attn_status = torch.zeros(4, dtype=torch.int32, device=query.device)
         return _lib.torch_ops().attention(
             query, key, value, idx.row_ptr, idx.bcsr_buf, None if idx.block_uniform else idx.raw_mask, self._attn_status,
-            numbers.rng, p, self._scale, numbers.seed, numbers.call, idx.block_nnz, self._Nt, self._Ns, self.check_status)
+            numbers.rng, p, self._scale, numbers.seed, numbers.call, idx.block_nnz, self._Nt, self._Ns, self._embed,
+            self.check_status)
 
     def forward_gathered(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                          out: torch.Tensor, copies: List[int]) -> torch.Tensor:
@@ -146,8 +144,8 @@ class SparseAttention(OperatorBase):
         assert self.ready and self._use_fused, 'forward_gathered needs an operator built on the fused kernel'
         return self._fused_forward(query.detach(), key.detach(), value.detach(), out=out, copies=copies)
 
-    def _fused_forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: Optional[torch.Tensor] = None,
-                       copies: Optional[List[int]] = None) -> torch.Tensor:
+    def _fused_forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                       copies: List[int]) -> torch.Tensor:
         _lib.require_cuda(q, k, v)
         idx = self._sparse_port.indexes
         shape = q.shape
@@ -156,10 +154,7 @@ class SparseAttention(OperatorBase):
         k = k.reshape(-1, self._Ns, E).contiguous()
         v = v.reshape(-1, self._Ns, E).contiguous()
         heads = q.shape[0]
-        if out is None:
-            out = torch.empty_like(q)
-        else:
-            assert out.is_contiguous() and out.dtype == q.dtype and out.numel() == q.numel() and out.device == q.device
+        assert out.is_contiguous() and out.dtype == q.dtype and out.numel() == q.numel() and out.device == q.device
         L = _lib.lib()
         ws_bytes = L.sparta_attn_fwd_workspace_bytes(heads, self._Nt, self._Ns, E, FUSED_BLOCK)
         if self._attn_ws is None or self._attn_ws.numel() < ws_bytes or self._attn_ws.device != q.device:
