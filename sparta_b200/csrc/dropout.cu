@@ -4,8 +4,8 @@
 // Bound by HBM: one read and one write per element, which leaves the SMs about 20 instructions per 16-bit element.  A
 // thread owns 16 bytes of 16-bit elements (32 of fp32), one call of the generator, at the same place of several rows:
 // the column's share of the generator is made once for all of them, the row's share once per row, and the decisions
-// are applied to packed pairs (with a full call and a compare and a select per element the kernel issued 23
-// instructions per element and took 119 us for 134 M bf16 elements; now see the table in the design notes).
+// are applied to packed pairs (134 M bf16 elements: 83 us, 99 % of the measured HBM rate, 13 instructions per element; with a
+// full call and a compare and a select per element 119 us and 23).
 // Rows whose length is no multiple of 8 begin anywhere in a 16-byte piece of memory.  Pieces stay aligned, so that a
 // piece holds the end of one group of eight columns and the beginning of the next: each lane makes the decisions of the
 // group that begins in its piece and takes those of the group before from the lane below (the lowest lane of a segment
