@@ -377,6 +377,7 @@ Tensor attention(const Tensor& query, const Tensor& key, const Tensor& value, co
   TORCH_CHECK_VALUE(k_heads == v_heads && k_heads > 0 && q_heads % k_heads == 0, q_heads, " query heads cannot share ", k_heads,
                     " key and ", v_heads, " value heads");
   TORCH_CHECK_VALUE(q_heads <= INT_MAX && Nt <= INT_MAX && Ns <= INT_MAX, "attention: a dimension beyond 31 bits");
+  TORCH_CHECK_VALUE(row_ptr.device() == query.device(), "the mask is on ", row_ptr.device(), ", the inputs on ", query.device());
   rng_pointer(rng, query);
   if (at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad()))
     return AttentionFn::apply(query, key, value, row_ptr, bcsr, mask, status, rng, p, scale,

@@ -47,7 +47,8 @@ class SparseAttention(OperatorBase):
         rotary: a ``RotaryEmbedding`` that turns queries and keys first.
 
     ``forward(query, key, value, rng=None, positions=None, key_positions=None)``: ``rng`` replaces the module's own
-    random numbers (see ``SparseDropout``), the positions go to ``rotary``.  Inputs are finite: a NaN or an infinity
+    random numbers (see ``SparseDropout``), the positions go to ``rotary``.  A mask with holes inside
+    its 64 x 64 blocks is read again by the fused backward pass: it may not be rewritten in between.  Inputs are finite: a NaN or an infinity
     in a row reaches, forward and backward, all rows that share a kept 64 x 64 block with it, masked elements of the block
     included, and those of that block's neighbour in the same 128 rows.
 

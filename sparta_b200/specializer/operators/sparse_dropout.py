@@ -33,8 +33,16 @@ class _Counter(object):
     """Host-side random state of a module: a seed and the number of training calls so far."""
 
     def __init__(self, seed: Optional[int]):
+        self.drawn = seed is None
         self.seed = int(torch.randint(0, 1 << 62, (), dtype=torch.int64)) if seed is None else int(seed)
         self.calls = 0
+
+    def __deepcopy__(self, memo) -> '_Counter':
+        """A copied layer is another layer: it drops other positions, unless its seed was chosen."""
+        copy = _Counter(None if self.drawn else self.seed)
+        if not self.drawn:
+            copy.calls = self.calls
+        return copy
 
     def next(self, rng: Optional[torch.Tensor]) -> DropoutKey:
         if rng is not None:
@@ -55,6 +63,8 @@ def sparse_dropout(x: torch.Tensor, p: float, key: DropoutKey, indexes: Optional
         raise ValueError('dropout of block values needs the BCSR indexes of one 2-D mask')
     if indexes.block_W < 8:
         raise ValueError(f'dropout of block values needs blocks at least 8 wide, got {indexes.block_W}')
+    if indexes.bcsr_buf.device != x.device:
+        raise ValueError(f'the indexes are on {indexes.bcsr_buf.device}, the input on {x.device}')
     if x.dim() == 0 or x.shape[-1] != indexes.val_stride_blocks * indexes.block_H * indexes.block_W:
         raise ValueError(f'the input of shape {tuple(x.shape)} does not hold the block values of these indexes')
     return _lib.torch_ops().dropout(x, p, key.rng, key.seed, key.call, indexes.bcsr_buf, indexes.nnz_dev, indexes.block_H,
@@ -70,15 +80,16 @@ class SparseDropout(torch.nn.Module):
 
     Args:
         p: probability that an element is dropped.
-        seed: 64-bit seed (default: drawn from torch's generator).  Modules with one seed drop alike.
+        seed: 64-bit seed (default: drawn from torch's generator, again for every deep copy of the module).  Modules
+            with one seed drop alike.
 
-    Shape: any shape, float32 / float16 / bfloat16; the last two dimensions are rows and columns, those before them
-    together the batch.  With ``indexes`` (``get_sparse_indexes()`` of an operator) the input holds block values
+    Shape: any shape (columns up to 2^30), float32 / float16 / bfloat16; the last two dimensions are rows and columns,
+    those before them together the batch.  With ``indexes`` (``get_sparse_indexes()`` of an operator) the input holds block values
     :math:`(*, nnz \cdot BH \cdot BW)`.
 
     ``forward(x, rng=None, indexes=None)``: without ``rng`` the module's seed and its count of calls select the
     numbers; ``rng``, an int64 tensor (seed, call number) on the GPU, replaces both and is what a captured graph
-    needs.  In evaluation mode, and for ``p == 0``, the input is returned.
+    needs, and a forward pass that is run again for its gradients (activation checkpointing).  In evaluation mode, and for ``p == 0``, the input is returned.
     """
 
     def __init__(self, p: float = 0.5, seed: Optional[int] = None):

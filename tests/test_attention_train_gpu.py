@@ -124,7 +124,8 @@ def test_forward_and_gradients(shape, dim, dtype):
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('dim', [64, 128])
 @pytest.mark.parametrize('p', [0.1, 0.75, 0.9999])
-@pytest.mark.parametrize('shape', [(2, 2, 256, 256, 0.6, False), (4, 2, 192, 448, 0.6, True), (2, 1, 512, 128, 1.0, False)])
+@pytest.mark.parametrize('shape', [(2, 2, 256, 256, 0.6, False), (4, 2, 192, 448, 0.6, True), (2, 1, 512, 128, 1.0, False),
+                                   (2, 1, 2048, 192, 0.8, True), (1, 1, 64, 4096, 0.9, False)])
 def test_dropout(shape, p, dim, dtype):
     heads, kv_heads, nt, ns, share, elements = shape
     q, k, v, do = inputs(dtype, heads, kv_heads, nt, ns, dim)
@@ -498,3 +499,36 @@ def test_random_state_travels_with_the_module():
     assert torch.equal(a(q.cuda(), k.cuda(), v.cuda()), b(q.cuda(), k.cuda(), v.cuda()))
     a.eval(), b.eval()
     assert torch.equal(a(q.cuda(), k.cuda(), v.cuda()), build(mask, q, k, v)(q.cuda(), k.cuda(), v.cuda()))
+
+
+def test_long_sequences_with_global_tokens():
+    """Tiles launched head by head (queries and keys beyond L2) and shared by several CTAs (global rows and columns):
+    two heads against 64 bits on the GPU, with the mask's blocks as elements."""
+    heads, n, dim = 16, 16384, 128
+    block = torch.zeros((n // 64, n // 64), dtype=torch.bool)
+    i = torch.arange(n // 64)
+    block |= (i[:, None] - i[None, :]).abs() <= 2
+    block[0], block[:, 0] = True, True
+    mask = block.cuda().to(torch.uint8).repeat_interleave(64, 0).repeat_interleave(64, 1)
+    d = torch.Generator(device='cuda').manual_seed(2)
+    q, do = (torch.randn((heads, n, dim), generator=d, device='cuda').bfloat16() for _ in range(2))
+    k, v = (torch.randn((heads // 2, n, dim), generator=d, device='cuda').bfloat16() for _ in range(2))
+    op = build(mask, q, k, v)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = op(*leaves)
+    got = (out,) + torch.autograd.grad(out, leaves, do)
+    kept = mask.bool()
+    for kv in (0, heads // 2 - 1):
+        h = slice(2 * kv, 2 * kv + 2)
+        kk, vv = k[kv].detach().double(), v[kv].detach().double()
+        parts = []
+        for a in range(2 * kv, 2 * kv + 2):
+            p = torch.softmax((q[a].detach().double() @ kk.T / dim ** 0.5).masked_fill(~kept, -math.inf), -1)
+            o, dv = p @ vv, p.T @ do[a].double()
+            ds = p * (do[a].double() @ vv.T - (o * do[a].double()).sum(-1, keepdim=True)) / dim ** 0.5
+            parts.append((o, ds @ kk, ds.T @ q[a].detach().double(), dv))
+        want = [torch.stack([x[j] for x in parts]) for j in range(4)]
+        want[2], want[3] = want[2].sum(0), want[3].sum(0)
+        for name, x, y in zip(('out', 'dq', 'dk', 'dv'), (got[0][h], got[1][h], got[2][kv], got[3][kv]), want):
+            rel = ((x.detach().double() - y).norm() / y.norm()).item()
+            assert rel <= 4 * torch.finfo(torch.bfloat16).eps / 2, f'{name} of head {kv}: {rel}'

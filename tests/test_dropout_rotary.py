@@ -68,6 +68,19 @@ def test_dropout_state_round_trip():
     assert SparseDropout(0.5)._counter.seed == first
 
 
+def test_copies_of_a_module_drop_other_positions():
+    import copy
+    import pickle
+    drawn, chosen = SparseDropout(0.5), SparseDropout(0.5, seed=3)
+    drawn._counter.calls = chosen._counter.calls = 5
+    one, other = copy.deepcopy(drawn), copy.deepcopy(drawn)
+    assert len({drawn._counter.seed, one._counter.seed, other._counter.seed}) == 3 and one._counter.calls == 0
+    same = copy.deepcopy(chosen)
+    assert (same._counter.seed, same._counter.calls) == (3, 5)
+    stored = pickle.loads(pickle.dumps(drawn))
+    assert (stored._counter.seed, stored._counter.calls) == (drawn._counter.seed, 5)
+
+
 @pytest.mark.parametrize('scaling', ['none', 'linear', 'ntk', 'yarn'])
 def test_rotary_frequencies(scaling):
     freq, magnitude = rotary_frequencies(64, 10000.0, scaling, 8.0, 4096)
