@@ -4,12 +4,13 @@
 // Bound by HBM: one read and one write per element, which leaves the SMs about 20 instructions per 16-bit element.  A
 // thread owns 16 bytes of 16-bit elements (32 of fp32), one call of the generator, at the same place of several rows:
 // the column's share of the generator is made once for all of them, the row's share once per row, and the decisions
-// are applied to packed pairs (134 M bf16 elements: 83 us, 99 % of the measured HBM rate, 13 instructions per element; with a
+// are applied to packed pairs (134 M bf16 elements: 82 us, 100 % of the measured HBM rate, 13 instructions per element; with a
 // full call and a compare and a select per element 119 us and 23).
 // Rows whose length is no multiple of 8 begin anywhere in a 16-byte piece of memory.  Pieces stay aligned, so that a
 // piece holds the end of one group of eight columns and the beginning of the next: each lane makes the decisions of the
 // group that begins in its piece and takes those of the group before from the lane below (the lowest lane of a segment
-// only makes them).  Pieces at either end of a row are handled element by element.
+// only makes them).  Pieces at either end of a row are stored element by element, in a loop of their own that has as many
+// loads in flight (one after the other: 54 us instead of 50).
 #include <type_traits>
 
 #include "philox.cuh"
@@ -17,7 +18,7 @@
 namespace sparta {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;  // blocks of 256 wait longer for their last warp (58 M elements in rows of 4093: 49 us against 47.5)
 template <typename T>
 constexpr int kBatch = 8 / sizeof(T);  // rows whose loads are in flight together: 64 bytes per thread
 constexpr int kMaxRows = 8; // rows per thread, or 1 where rows are few
@@ -61,6 +62,12 @@ __device__ __forceinline__ void drop_pair(Piece<T>& p, int i, uint32_t mask, flo
   }
 }
 
+// the signs of the halves of two words, each over a byte
+__device__ __forceinline__ uint32_t spread4(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("prmt.b32 %0, %1, %2, 0xfdb9;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
 // The masks of a piece's four pairs.  Rows that are no multiple of 8 long begin `a` elements into a piece: the piece then
 // holds the last `a` columns of the group before the lane's own (whose decisions the lane below made) and the first
 // 8 - a of its own.  Every lane of the warp calls it.
@@ -73,22 +80,22 @@ __device__ __forceinline__ void piece_masks(const PhiloxKey& key, const PhiloxRo
 #pragma unroll
     for (int i = 0; i < 4; ++i) mask[i] = spread2(not_below2(w[i], t2));
   } else {
-    uint32_t own = 0;  // decisions of columns 2 i, 2 i + 1 at bits 2 i, 2 i + 16, then side by side
-#pragma unroll
-    for (int i = 0; i < 4; ++i) own |= (not_below2(w[i], t2) >> (15 - 2 * i)) & (0x00010001u << (2 * i));
-    own = (own | (own >> 15)) & 0xffu;
-    const uint32_t before = __shfl_up_sync(0xffffffffu, own, 1, seg);
-    uint32_t bits = (before | (own << 8)) >> (8 - a);
-    bits |= bits << 15;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mask[i] = spread2(bits << (15 - 2 * i));
+    // one byte per column, 0 or 255
+    const uint32_t own0 = spread4(not_below2(w[0], t2), not_below2(w[1], t2)), own1 = spread4(not_below2(w[2], t2), not_below2(w[3], t2));
+    const uint32_t before0 = __shfl_up_sync(0xffffffffu, own0, 1, seg), before1 = __shfl_up_sync(0xffffffffu, own1, 1, seg);
+    // bytes 8 - a .. 15 - a of before0, before1, own0, own1: shifted left by a bytes, 4 of them as whole words
+    const bool far = a >= 4;
+    const uint32_t n0 = far ? before0 : before1, n1 = far ? before1 : own0, n2 = far ? own0 : own1;
+    const uint32_t lo = __funnelshift_l(n0, n1, 8 * a), hi = __funnelshift_l(n1, n2, 8 * a);  // the shift is taken mod 32
+    mask[0] = __byte_perm(lo, 0, 0x1100); mask[1] = __byte_perm(lo, 0, 0x3322);
+    mask[2] = __byte_perm(hi, 0, 0x1100); mask[3] = __byte_perm(hi, 0, 0x3322);
   }
 }
 
 // Dense [rows, W], rows = batch * H; y 16-byte aligned, VEC: x too.  EVEN: W % 8 == 0.  A warp is 32 >> log_seg segments
 // of 1 << log_seg lanes, each on a row of its own; rows longer than a segment reaches are cut into `chunks`.
 template <typename T, bool EVEN, bool VEC>
-__global__ void __launch_bounds__(kThreads, 4)  // 64 registers: the loads of many warps hide each other
+__global__ void __launch_bounds__(kThreads, 8)  // 64 registers: the loads of many warps hide each other
 dropout_dense_kernel(const T* __restrict__ x, T* __restrict__ y, long long rows, int H, int W, int log_seg, int chunks,
                      int per_thread, DropoutParams d) {
   const PhiloxKey key = load_uniform_philox_key(d);
@@ -113,38 +120,55 @@ dropout_dense_kernel(const T* __restrict__ x, T* __restrict__ y, long long rows,
       col = philox_col(key, m, b);
     }
   };
-  if (d.threshold < kDropoutOne && (EVEN || m0 >= 0) && m0 + seg <= W / kPiece && per_thread >= kBatch<T> && W <= (1 << 24) &&
-      row0 + per_thread * per_warp <= rows) {
-    // ---- every piece of the warp is whole: loads of four rows in flight ----
-    // rows that begin anywhere: 32-bit offsets from the first one (58 M fp16 elements in rows of 4093: 61 -> 55 us); the
+  const bool inside = (EVEN || m0 >= 0) && m0 + seg <= W / kPiece;  // no piece of the warp holds an end of a row
+  if (d.threshold < kDropoutOne && (inside || (!EVEN && W >= kPiece)) && per_thread >= kBatch<T> && W <= (1 << 24) &&
+      (row0 + per_thread * per_warp < rows || (inside && row0 + per_thread * per_warp == rows))) {
+    // ---- all rows are there, and pieces may be read whole: loads of four rows in flight ----
+    // rows that begin anywhere: 32-bit offsets from the first one (58 M fp16 elements in rows of 4093: 61 -> 55 us when it was measured); the
     // other rows measured faster with 64-bit ones (134 M bf16 elements: 85 us against 93)
     using Offset = typename std::conditional<EVEN, long long, uint32_t>::type;
     const Offset step = static_cast<Offset>(per_warp) * static_cast<Offset>(W);
     const long long first = row * W;
-    Offset start = EVEN ? 0 : static_cast<Offset>(first & 7);
+    Offset start0 = EVEN ? 0 : static_cast<Offset>(first & 7);
     const long long base = ((first >> 3) + m) * kPiece;
     const T* px = x + base;
     T* py = y + base;
+    auto run = [&](auto ends) {
+      Offset start = start0;
 #pragma unroll 1
-    for (int k0 = 0; k0 < per_thread; k0 += kBatch<T>) {
-      Piece<T> in[kBatch<T>];
+      for (int k0 = 0; k0 < per_thread; k0 += kBatch<T>) {
+        Piece<T> in[kBatch<T>];
 #pragma unroll
-      for (int k = 0; k < kBatch<T>; ++k)
-        if (!makes_only) in[k] = load_piece<T, VEC>(px + (EVEN ? start + k * step : (start + k * step) / kPiece * kPiece));
+        for (int k = 0; k < kBatch<T>; ++k) {
+          const Offset s = start + k * step;
+          const bool read = !makes_only && (!ends || kPiece * m - static_cast<int>(s & 7) < W);
+          if (read) in[k] = load_piece<T, VEC>(px + (EVEN ? s : s / kPiece * kPiece));
+        }
 #pragma unroll
-      for (int k = 0; k < kBatch<T>; ++k) {
-        uint32_t mask[4];
-        piece_masks<EVEN>(key, philox_row(key, r, b), col, t2, static_cast<int>(start) & 7, seg, mask);
+        for (int k = 0; k < kBatch<T>; ++k) {
+          uint32_t mask[4];
+          piece_masks<EVEN>(key, philox_row(key, r, b), col, t2, static_cast<int>(start) & 7, seg, mask);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) drop_pair(in[k], i, mask[i], d.scale);
-        if (!makes_only) store_piece(py + (EVEN ? start : start / kPiece * kPiece), in[k]);
-        start += step;
-        next_row();
+          for (int i = 0; i < 4; ++i) drop_pair(in[k], i, mask[i], d.scale);
+          T* out = py + (EVEN ? start : start / kPiece * kPiece);
+          const int c0 = kPiece * m - static_cast<int>(start & 7);  // column of the piece's first element
+          if (!ends || (c0 >= 0 && c0 + kPiece <= W)) {
+            if (!makes_only) store_piece(out, in[k]);
+          } else if (!makes_only) {
+#pragma unroll
+            for (int i = 0; i < kPiece; ++i)
+              if (c0 + i >= 0 && c0 + i < W) out[i] = in[k].v[i];
+          }
+          start += step;
+          next_row();
+        }
       }
-    }
+    };
+    if (EVEN || inside) run(std::false_type{});
+    else run(std::true_type{});
     return;
   }
-  // ---- ends of rows, the last rows, and p = 1: piece by piece, whole or in part ----
+  // ---- the last rows, few rows, and p = 1: piece by piece, whole or in part ----
 #pragma unroll 1
   for (int k = 0; k < per_thread; ++k, row += per_warp) {
     const long long start = row * W;

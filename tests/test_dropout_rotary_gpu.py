@@ -49,6 +49,26 @@ def test_dropout_forward_and_backward(shape, dtype):
         close(got, src.double() * keep * oracle.dropout_scale(p), dtype)
 
 
+# Many rows, so that a thread takes several of them: segments of a warp on rows of their own, rows in several chunks, a
+# change of batch element inside a thread's rows, ends of rows within and at the end of the tensor, an odd first address.
+MANY = [(3, 50700, 9), (2, 4740, 257), (1, 3792, 1001), (2, 37900, 64), (19000, 8, 11), (1, 152000, 8), (5, 30001, 7)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape', MANY)
+@pytest.mark.parametrize('offset', [0, 3])
+def test_dropout_of_many_rows(shape, offset, dtype):
+    n = shape[0] * shape[1] * shape[2]
+    g = torch.Generator(device='cuda').manual_seed(2)
+    x = torch.randn(n + offset, generator=g, device='cuda').to(dtype)[offset:].view(shape)
+    p, seed, call = 0.2, 99, 3
+    keep = oracle.dropout_keep(seed, call, *shape, p)
+    y = SparseDropout(p)(x, rng=rng(seed, call))
+    want = x.double().cpu() * keep * oracle.dropout_scale(p)
+    assert torch.equal(y.cpu() != 0, keep & (x.cpu() != 0))
+    close(y, want, dtype)
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('offset,cols', [(1, 64), (3, 61), (8, 64), (5, 8)])
 def test_dropout_of_unaligned_and_strided_inputs(offset, cols, dtype):
