@@ -69,17 +69,25 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float v0, float v1) {
 // 0xffff in each half whose bit (i, 16 + i) is set
 __device__ __forceinline__ uint32_t pair_mask(uint32_t word, int i) { return spread2(word << (15 - i)); }
 
-// 32 dropout decisions of columns 32 g .. of a row, split order
-__device__ __forceinline__ uint32_t philox_split32(const PhiloxKey& key, const PhiloxRow& r, uint32_t t2, uint32_t g, uint32_t batch) {
-  uint32_t bits = 0;
+// 32 dropout decisions of columns 32 g .. of a row: column c at bit c (IN_ORDER), or at bit drop_bit(c), which takes
+// half the instructions.  Decisions come as masks of bytes; a product of four bytes with powers of two sums them up.
+__device__ __forceinline__ constexpr int drop_bit(int c) { return 8 * (c & 3) + (c >> 2); }
+template <bool IN_ORDER>
+__device__ __forceinline__ uint32_t philox_bits32(const PhiloxKey& key, const PhiloxRow& r, uint32_t t2, uint32_t g, uint32_t batch) {
+  uint32_t part[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint32_t w[4];
     philox8(key, r, philox_col(key, 4 * g + q, batch), w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bits = (bits >> 1) | (not_below2(w[i], t2) & 0x80008000u);
+    const uint32_t lo = spread4(not_below2(w[0], t2), not_below2(w[1], t2)), hi = spread4(not_below2(w[2], t2), not_below2(w[3], t2));
+    if constexpr (IN_ORDER) {  // bytes are 0 or -1: times -1, -2, -4 .. -128
+      part[q] = __dp4a(static_cast<int>(hi), static_cast<int>(0x80c0e0f0u), __dp4a(static_cast<int>(lo), static_cast<int>(0xf8fcfeffu), 0));
+    } else {
+      part[q] = (lo & (0x01010101u << (2 * q))) | (hi & (0x02020202u << (2 * q)));
+    }
   }
-  return bits;
+  if constexpr (IN_ORDER) return __byte_perm(__byte_perm(part[0], part[1], 0x0040), __byte_perm(part[2], part[3], 0x0040), 0x5410);
+  return (part[0] | part[1]) | (part[2] | part[3]);
 }
 // packed pairs of columns 32 g .. of a row: the dropped ones to zero
 __device__ __forceinline__ void drop_packed32(uint32_t* packed, const PhiloxKey& key, const PhiloxRow& r, uint32_t t2, uint32_t g, uint32_t batch) {
@@ -106,7 +114,7 @@ __device__ __forceinline__ uint32_t mask_word32(const uint8_t* m) {
   return bits;
 }
 
-// the even bits gathered in the lower half, the odd ones in the upper, and back
+// the even bits gathered in the lower half, the odd ones in the upper
 __device__ __forceinline__ uint32_t split_bits32(uint32_t x) {
   uint32_t t;
   t = (x ^ (x >> 1)) & 0x22222222u; x ^= t ^ (t << 1);
@@ -115,13 +123,4 @@ __device__ __forceinline__ uint32_t split_bits32(uint32_t x) {
   t = (x ^ (x >> 8)) & 0x0000ff00u; x ^= t ^ (t << 8);
   return x;
 }
-__device__ __forceinline__ uint32_t unsplit_bits32(uint32_t x) {
-  uint32_t t;
-  t = (x ^ (x >> 8)) & 0x0000ff00u; x ^= t ^ (t << 8);
-  t = (x ^ (x >> 4)) & 0x00f000f0u; x ^= t ^ (t << 4);
-  t = (x ^ (x >> 2)) & 0x0c0c0c0cu; x ^= t ^ (t << 2);
-  t = (x ^ (x >> 1)) & 0x22222222u; x ^= t ^ (t << 1);
-  return x;
-}
-
 }  // namespace sparta

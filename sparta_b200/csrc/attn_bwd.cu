@@ -519,7 +519,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
       const int blk = e >> 2;
       const uint32_t s_addr = s_base + (j % kSBuf) * C::kCols;
       // words of decisions over the warp's 32 x 32 scores, made for rows of the score matrix: for this thread's own over
-      // its columns (split order), or for query `lane` of the block over the warp's keys
+      // its columns (mask: split order, dropout: drop_bit()), or for query `lane` of the block over the warp's keys
       uint32_t mask_w = 0xffffffffu, keep_w = 0xffffffffu;
       if ((MASK || DROP) && mine) {
         const int q_row = DKV ? blk * kBlk + (quarter & 1) * 32 + lane : grow;
@@ -531,8 +531,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
         if constexpr (DROP) {
           const int q_head = DKV ? head * p.group + h : head;
           if constexpr (DKV) key_row = philox_row(key, q_row, q_head);
-          keep_w = philox_split32(key, key_row, t2, word, q_head);
-          if constexpr (DKV) keep_w = unsplit_bits32(keep_w);
+          keep_w = philox_bits32<DKV>(key, key_row, t2, word, q_head);
         }
       }
       if (++k == pairs) { k = 0; ++h; }
@@ -621,8 +620,8 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
             for (int r = 0; r < 4; ++r) {
               const int i = (r >> 1) * 8 + 2 * n + (r & 1);
               float2 v = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-              if constexpr (DROP) v = mask_pair(mul2(v, up2), d, r);
-              v = mul2(prob[i], add2(v, stats));
+              v = DROP ? fma2(mask_pair(v, d, r), up2, stats) : add2(v, stats);
+              v = mul2(prob[i], v);
               packed[i] = pack2<T>(v.x, v.y);
               // a masked score's probability is zero, and so is its dS whatever stands in V
               if constexpr (MASK) packed[i] &= packed_mask(m, r);
@@ -633,11 +632,10 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
           for (int i = 0; i < 16; ++i) {
             float2 v = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
             if constexpr (DROP) {
-              v = mul2(v, up2);
-              v.x = (keep_w >> i) & 1u ? v.x : 0.f;
-              v.y = (keep_w >> (i + 16)) & 1u ? v.y : 0.f;
+              v.x = (keep_w >> drop_bit(2 * i)) & 1u ? v.x : 0.f;
+              v.y = (keep_w >> drop_bit(2 * i + 1)) & 1u ? v.y : 0.f;
             }
-            v = mul2(prob[i], add2(v, nd));
+            v = mul2(prob[i], DROP ? fma2(v, up2, nd) : add2(v, nd));
             packed[i] = pack2<T>(v.x, v.y);
             if constexpr (MASK) packed[i] &= pair_mask(mask_w, i);
           }

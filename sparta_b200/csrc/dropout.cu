@@ -62,12 +62,6 @@ __device__ __forceinline__ void drop_pair(Piece<T>& p, int i, uint32_t mask, flo
   }
 }
 
-// the signs of the halves of two words, each over a byte
-__device__ __forceinline__ uint32_t spread4(uint32_t a, uint32_t b) {
-  uint32_t m;
-  asm("prmt.b32 %0, %1, %2, 0xfdb9;" : "=r"(m) : "r"(a), "r"(b));
-  return m;
-}
 // The masks of a piece's four pairs.  Rows that are no multiple of 8 long begin `a` elements into a piece: the piece then
 // holds the last `a` columns of the group before the lane's own (whose decisions the lane below made) and the first
 // 8 - a of its own.  Every lane of the warp calls it.

@@ -105,6 +105,12 @@ __device__ __forceinline__ uint32_t spread2(uint32_t x) {
   asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(m) : "r"(x));  // sign of byte 1, byte 3 over two bytes each
   return m;
 }
+// bits 15 and 31 of two words, each over a byte, lower columns in lower bytes
+__device__ __forceinline__ uint32_t spread4(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("prmt.b32 %0, %1, %2, 0xfdb9;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
 // The threshold in both halves.  "Everything dropped" (65536) becomes "nothing": its scale is 0.
 __device__ __forceinline__ uint32_t threshold2(const DropoutParams& d) { return (d.threshold & 0xffffu) * 0x00010001u; }
 
