@@ -256,6 +256,8 @@ int sparta_attn_fwd_gather(const void* Q, const void* K, const void* V, void* O,
  *   dropout in [0, 1], rng / seed / call as for sparta_dropout.
  *   nnz_hint: kept blocks of the mask as far as the host knows (0: unknown); decides only how the backward pass divides
  *   its work over the GPU.  workspace (backward only): sparta_attn_train_bwd_workspace_bytes(), 16-byte aligned, no initial contents.
+ *   With dropout, sparta_attn_train_bwd_dropout_bytes() more (a bit per kept score, 1 GiB at most) let both gradient
+ *   passes read decisions that are made once; without room for those of all kept blocks each pass makes its own.
  */
 typedef struct sparta_attn_train_args {
   const void* Q;
@@ -284,6 +286,8 @@ typedef struct sparta_attn_train_args {
 int sparta_attn_train_fwd(const sparta_attn_train_args* h_args, void* stream);
 
 size_t sparta_attn_train_bwd_workspace_bytes(int heads, int kv_heads, int Nt, int Ns, int D, int64_t nnz_hint);
+
+size_t sparta_attn_train_bwd_dropout_bytes(int heads, int64_t nnz_hint);
 
 int sparta_attn_train_bwd(const sparta_attn_train_args* h_args, void* stream);
 

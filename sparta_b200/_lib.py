@@ -103,6 +103,7 @@ SIGNATURES = {
                                        c_void_p, POINTER(c_void_p), c_int, c_void_p]),
     'sparta_attn_train_fwd': (c_int, [POINTER(AttnTrainArgs), c_void_p]),
     'sparta_attn_train_bwd_workspace_bytes': (c_size_t, [c_int] * 5 + [c_int64]),
+    'sparta_attn_train_bwd_dropout_bytes': (c_size_t, [c_int, c_int64]),
     'sparta_attn_train_bwd': (c_int, [POINTER(AttnTrainArgs), c_void_p]),
     'sparta_dropout': (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_double, c_void_p, c_uint64, c_uint64,
                                c_int, c_void_p]),

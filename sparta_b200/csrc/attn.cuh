@@ -18,6 +18,7 @@ struct AttnArgs {
   void* dK;
   void* dV;
   void* workspace;
+  size_t workspace_bytes;
   const int32_t* row_ptr;
   const int32_t* idx;
   const uint8_t* mask;      // [Nt, Ns] element mask or null
@@ -38,6 +39,7 @@ int attn_tc64_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* stat
 
 // backward pass (attn_bwd.cu)
 size_t attn_bwd_workspace(int heads, int kv_heads, int Nt, int Ns, int D, long long nnz);
+size_t attn_bwd_dropout_workspace(int heads, long long nnz);
 int attn_bwd_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* status, cudaStream_t st);
 
 // 2^x by the special-function unit alone.  exp2f() wraps the same instruction in a range fix for
@@ -69,24 +71,17 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float v0, float v1) {
 // 0xffff in each half whose bit (i, 16 + i) is set
 __device__ __forceinline__ uint32_t pair_mask(uint32_t word, int i) { return spread2(word << (15 - i)); }
 
-// 32 dropout decisions of columns 32 g .. of a row: column c at bit c (IN_ORDER), or at bit drop_bit(c), which takes
-// half the instructions.  Decisions come as masks of bytes; a product of four bytes with powers of two sums them up.
-__device__ __forceinline__ constexpr int drop_bit(int c) { return 8 * (c & 3) + (c >> 2); }
-template <bool IN_ORDER>
+// 32 dropout decisions of columns 32 g .. of a row, column c at bit 7 - c / 4 of byte c % 4: shifted left by u, the signs of
+// the four bytes are columns 4 u .. 4 u + 3.
 __device__ __forceinline__ uint32_t philox_bits32(const PhiloxKey& key, const PhiloxRow& r, uint32_t t2, uint32_t g, uint32_t batch) {
   uint32_t part[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint32_t w[4];
     philox8(key, r, philox_col(key, 4 * g + q, batch), w);
-    const uint32_t lo = spread4(not_below2(w[0], t2), not_below2(w[1], t2)), hi = spread4(not_below2(w[2], t2), not_below2(w[3], t2));
-    if constexpr (IN_ORDER) {  // bytes are 0 or -1: times -1, -2, -4 .. -128
-      part[q] = __dp4a(static_cast<int>(hi), static_cast<int>(0x80c0e0f0u), __dp4a(static_cast<int>(lo), static_cast<int>(0xf8fcfeffu), 0));
-    } else {
-      part[q] = (lo & (0x01010101u << (2 * q))) | (hi & (0x02020202u << (2 * q)));
-    }
+    part[q] = (spread4(not_below2(w[0], t2), not_below2(w[1], t2)) & (0x80808080u >> (2 * q))) |
+              (spread4(not_below2(w[2], t2), not_below2(w[3], t2)) & (0x40404040u >> (2 * q)));
   }
-  if constexpr (IN_ORDER) return __byte_perm(__byte_perm(part[0], part[1], 0x0040), __byte_perm(part[2], part[3], 0x0040), 0x5410);
   return (part[0] | part[1]) | (part[2] | part[3]);
 }
 // packed pairs of columns 32 g .. of a row: the dropped ones to zero

@@ -1,5 +1,6 @@
 // Backward pass of the fused block-sparse attention (fp16 / bf16, head dim 64 or 128, 64 x 64 mask blocks).  The
-// probabilities are recomputed from Q, K and the forward pass's row log-sum-exp; nothing of size Nt x Ns is stored.
+// probabilities are recomputed from Q, K and the forward pass's row log-sum-exp; nothing of size Nt x Ns is stored
+// but, with dropout and for the time of the call, a bit per kept score.
 //
 //   S = Q K^T    P = exp(scale S - lse)            on kept elements, 0 elsewhere
 //   P' = P keep up                                  (dropout: keep in {0, 1}, up = 1 / (1 - p))
@@ -43,7 +44,9 @@
 // therefore reads and writes tensor memory in the fragment layout, where a thread has four rows and eight columns.
 //
 // Masks and dropout are words of 32 decisions per row of the score matrix (query): in the dQ pass each thread's own, in
-// the dK, dV pass each lane makes one and the threads fetch those of their eight columns from the lanes that made them.
+// the dK, dV pass each lane has one and the threads fetch those of their eight columns from the lanes that have them.
+// Dropout decisions are made once, by the first kernel, for both passes, if the workspace has room (B4 H16 S4096 D64,
+// p = 0.1: 716 us with the generator in the steps of both; 621 us now, of which 95 the first kernel, 520 the passes).
 // The forward pass it belongs to: SparseAttention.forward (sparta/specializer/operators/sparse_attention.py:76-80),
 // whose gradients the reference takes through its three operators.
 #include <type_traits>
@@ -71,7 +74,12 @@ struct BwdParams {
   float scale, scale_log2;
   int32_t* status;
   DropoutParams drop;
+  const int32_t* position;  // [Nt / 64, present_pitch]: place of a kept block in the index (dropout only)
+  const uint32_t* bits;     // [heads, bits_blocks, 2, 64]: decisions by place in the index, made by the first
+  int bits_blocks;          // kernel; 32 columns of a query row per word
+  const int32_t* blocks;    // kept blocks: where they are more than bits_blocks, decisions are made in the steps
 };
+constexpr int kBitWords = kBlk * kBlk / 32;  // of a block
 
 struct PassParams {         // of one of the two passes
   void* out1;               // dQ, or dK
@@ -101,7 +109,9 @@ struct BwdCfg {
   static constexpr uint32_t kAcc1 = kDpCol + kCols, kAcc2 = kAcc1 + D;
   static constexpr uint32_t kTmemCols = 512 / kCtasPerSM;
   static_assert(kAcc2 + (DKV ? D : 0) <= kTmemCols, "tensor memory budget");
-  static constexpr int kSmem = 2 * kABytes + kStages * (2 * kBBytes + kStatFloats * 4) + kMaxBlocks * 3 + 512 + 1024;
+  static constexpr int smem_bytes(bool drop) {
+    return 2 * kABytes + kStages * (2 * kBBytes + kStatFloats * 4) + (drop ? 2 * kMaxBlocks * 4 : 0) + kMaxBlocks * 3 + 512 + 1024;
+  }
 };
 
 // two 32-bit operations in one instruction
@@ -149,24 +159,79 @@ __device__ __forceinline__ float2 mask_pair(float2 v, const ColumnMasks& m, int 
                      __uint_as_float(__float_as_uint(v.y) & permute_signs(m.c1, 0, 0x8888u + r * 0x1111u)));
 }
 
+// Dropout decisions of a 32 x 32 region for a thread of the fragment layout, from the lanes' words of a column each
+// (philox_bits32, its columns the region's rows): column pair n in byte n, rows lane / 4 + 8 r at bits 7 - 2 r of the first
+// column and 6 - 2 r of the second.  A shift by 2 r thus has row r's decisions at the tops of the bytes.
+__device__ __forceinline__ uint32_t fragment_bits(uint32_t word, int lane) {
+  const int g = lane >> 2, turn = 8 * (g & 3) - (g >> 2);  // brings row 8 r + g to bit 7 - 2 r
+  uint32_t pair[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const uint32_t c0 = __shfl_sync(0xffffffffu, word, 8 * n + 2 * (lane & 3)), c1 = __shfl_sync(0xffffffffu, word, 8 * n + 2 * (lane & 3) + 1);
+    pair[n] = (__funnelshift_r(c0, c0, turn) & 0xaau) | (__funnelshift_r(c1, c1, turn + 1) & 0x55u);
+  }
+  return __byte_perm(__byte_perm(pair[0], pair[1], 0x0040), __byte_perm(pair[2], pair[3], 0x0040), 0x5410);
+}
+
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
 
-// The negated delta and log-sum-exp of every query row; the blocks kept, as bytes, for the pass that walks columns.
-// Bound by the read of O and dO.  A row is D / 8 lanes of 16 bytes; four rows' loads are in flight per thread.
+// The dropout decisions of all blocks of the index and all heads, if there is room.  A warp makes a block's, two rows
+// per lane, so that the columns' share of the generator serves both.  Bound by the integer instructions, about 45 per call
+// of the generator: 334 M decisions in 83 us.
+__device__ void make_dropout_bits(const DropoutParams& drop, const int32_t* __restrict__ idx, int blocks, int bits_blocks, int heads,
+                                  uint32_t* __restrict__ bits, uint32_t warp, uint32_t warps) {
+  const int lane = threadIdx.x & 31;
+  const PhiloxKey key = load_uniform_philox_key(drop);
+  const uint32_t t2 = threshold2(drop);
+  if (blocks > bits_blocks) return;  // they will be made in the steps
+  const uint32_t n = max(0, blocks);
+  for (uint64_t item = warp; item < static_cast<uint64_t>(n) * heads; item += warps) {
+    const uint32_t head = static_cast<uint32_t>(item / n), e = static_cast<uint32_t>(item - static_cast<uint64_t>(head) * n);
+    const uint32_t entry = static_cast<uint32_t>(__ldg(idx + e));
+    const uint32_t row = (entry >> 16) * kBlk + lane, word = (entry & 0xffffu) * (kBlk / 32);
+    uint32_t* dst = bits + (static_cast<uint64_t>(head) * bits_blocks + e) * kBitWords + lane;
+    const PhiloxRow r0 = philox_row(key, row, head), r1 = philox_row(key, row + 32, head);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      dst[w * kBlk] = philox_bits32(key, r0, t2, word + w, head);
+      dst[w * kBlk + 32] = philox_bits32(key, r1, t2, word + w, head);
+    }
+  }
+}
+
+// The negated delta and log-sum-exp of every query row; the blocks kept, as bytes, for the pass that walks columns; their
+// places in the index and their dropout decisions.  The latter are arithmetic, for which the first `bits_ctas` CTAs are
+// there; the rest is bound by the read of O and dO.  A row is D / 8 lanes of 16 bytes; four rows' loads are in flight per
+// thread.
 constexpr int kPrepRows = 4;
-template <typename T, int D>
+struct PrepBits {
+  DropoutParams drop;
+  int32_t* position;
+  uint32_t* bits;
+  int blocks, heads, ctas;
+};
+template <typename T, int D, bool DROP>
 __global__ void __launch_bounds__(256)
 attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const float* __restrict__ lse, float* __restrict__ neg_lse,
                      float* __restrict__ neg_delta, uint8_t* __restrict__ present, const int32_t* __restrict__ row_ptr,
                      const int32_t* __restrict__ idx, long long rows, int nbr, int nbc, int pitch,
-                     uint32_t* __restrict__ tickets, long long n_tickets) {
+                     uint32_t* __restrict__ tickets, long long n_tickets, const __grid_constant__ PrepBits make) {
+  int block = blockIdx.x, grid = gridDim.x;
+  if constexpr (DROP) {
+    if (block < make.ctas) {
+      make_dropout_bits(make.drop, idx, __ldg(row_ptr + nbr), make.blocks, make.heads, make.bits, block * 8 + (threadIdx.x >> 5), make.ctas * 8);
+      return;
+    }
+    block -= make.ctas;
+    grid -= make.ctas;
+  }
   constexpr int kLanes = D / 8, kStep = 256 / kLanes;
   const int lane = threadIdx.x % kLanes;
-  const long long row0 = (long long)blockIdx.x * (kPrepRows * kStep) + threadIdx.x / kLanes;
+  const long long row0 = (long long)block * (kPrepRows * kStep) + threadIdx.x / kLanes;
   uint4 a[kPrepRows], b[kPrepRows];
 #pragma unroll
   for (int k = 0; k < kPrepRows; ++k) {
@@ -193,15 +258,18 @@ attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const fl
       neg_lse[row] = lse[row] == -INFINITY ? -INFINITY : lse[row] * -1.4426950408889634f;
     }
   }
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n_tickets; i += (long long)gridDim.x * 256) tickets[i] = 0;
+  for (long long i = (long long)block * 256 + threadIdx.x; i < n_tickets; i += (long long)grid * 256) tickets[i] = 0;
   __shared__ uint8_t kept[kMaxBlocks];
-  for (int r = blockIdx.x; r < nbr; r += gridDim.x) {  // block rows of the mask
+  for (int r = block; r < nbr; r += grid) {  // block rows of the mask
     __syncthreads();
     for (int c = threadIdx.x; c < pitch; c += 256) kept[c] = 0;
     __syncthreads();
     for (int e = row_ptr[r] + threadIdx.x; e < row_ptr[r + 1]; e += 256) {
       const int c = __ldg(idx + e) & 0xffff;
-      if (c < nbc) kept[c] = 1;  // index arrays come from the caller: never index shared memory with them unchecked
+      if (c < nbc) {  // index arrays come from the caller: never index shared memory with them unchecked
+        kept[c] = 1;
+        if constexpr (DROP) make.position[(long long)r * pitch + c] = e;
+      }
     }
     __syncthreads();
     for (int c = threadIdx.x; c < pitch; c += 256) present[(long long)r * pitch + c] = kept[c];
@@ -210,7 +278,8 @@ attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const fl
 
 // SPLIT: several CTAs may share a tile.  A variant of its own, because the other one keeps its registers for the steps
 // (B4 H16 S4096 D64, which does not split: 509 us with the code for it, 483 us without).
-template <bool DKV, int D, int FMT, bool MASK, bool DROP, bool SPLIT>
+// READY: the first kernel has made every block's dropout decisions (otherwise they are made in the steps).
+template <bool DKV, int D, int FMT, bool MASK, bool DROP, bool READY, bool SPLIT>
 __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtensorMap& tm_a2, const CUtensorMap& tm_b1,
                                          const CUtensorMap& tm_b2, const BwdParams& p, const PassParams& pass, int block) {
   using T = typename std::conditional<FMT == 0, __half, __nv_bfloat16>::type;
@@ -225,7 +294,8 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
   uint8_t* b1_s = a2_s + C::kABytes;                        // [kStages]
   uint8_t* b2_s = b1_s + kStages * C::kBBytes;              // [kStages]
   float* stat_s = reinterpret_cast<float*>(b2_s + kStages * C::kBBytes);  // [kStages][neg_lse, neg_delta of the step's columns]
-  uint16_t* ulist = reinterpret_cast<uint16_t*>(stat_s + kStages * C::kStatFloats);  // (block << 2) | presence bits
+  int32_t* pos_s = reinterpret_cast<int32_t*>(stat_s + kStages * C::kStatFloats);    // [2][kMaxBlocks] offsets of decisions
+  uint16_t* ulist = reinterpret_cast<uint16_t*>(pos_s + (DROP ? 2 * kMaxBlocks : 0));  // (block << 2) | presence bits
   uint8_t* kmask = reinterpret_cast<uint8_t*>(ulist + kMaxBlocks);
   uint64_t* a1_full = reinterpret_cast<uint64_t*>(kmask + kMaxBlocks);
   uint64_t* a2_full = a1_full + 1;
@@ -316,6 +386,17 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
   tc_fence_after_sync();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_holder, 0);
   const int count = __shfl_sync(0xffffffffu, *s_count, 0);
+  if constexpr (READY) {
+    for (int i = threadIdx.x; i < 2 * count; i += kThreads) {
+      const int half = i & 1, e = ulist[i >> 1], blk = e >> 2;
+      if ((e >> half) & 1) {
+        const int pos = __ldg(p.position + (DKV ? (long long)blk * p.present_pitch + blk0 + half
+                                                : (long long)(blk0 + half) * p.present_pitch + blk));
+        pos_s[half * kMaxBlocks + (i >> 1)] = pos * kBitWords;
+      }
+    }
+    __syncthreads();
+  }
   const int pairs = (count + C::kBlocks - 1) / C::kBlocks;  // steps through the list
   const int all_steps = DKV ? pairs * p.group : pairs;  // dK, dV: the list once for every head that shares the keys
   // A tile whose steps would take one CTA far longer than the others (global tokens, heads that share their keys), or
@@ -500,26 +581,41 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
       nl.x = nl.y = __ldg(p.neg_lse + a_row0 + row);
       nd.x = nd.y = __ldg(p.neg_delta + a_row0 + row);
     }
-    PhiloxKey key = {};
-    PhiloxRow key_row = {};
-    if constexpr (DROP) {
-      key = load_uniform_philox_key(p.drop);
-      if constexpr (!DKV) key_row = philox_row(key, grow, head);
-    }
-    const uint32_t t2 = threshold2(p.drop);
     const float up = p.drop.scale;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     int h = h0, k = k0;
+    // READY: the list entry of a step and the decisions of its 32 x 32 scores, a step ahead
+    const uint32_t* bits = nullptr;  // of the head, for this thread
+    uint32_t next_bits = 0;
+    int next_e = 0;
+    auto look_ahead = [&] {
+      const int at = C::kBlocks * k + (quarter >> 1);
+      next_e = __shfl_sync(0xffffffffu, at < count ? ulist[at] : 0, 0);
+      if ((next_e >> half) & 1) next_bits = __ldg(bits + pos_s[half * kMaxBlocks + at]);
+    };
+    PhiloxKey key = {};
+    PhiloxRow key_row = {};
+    if constexpr (DROP && !READY) {
+      key = load_uniform_philox_key(p.drop);
+      if constexpr (!DKV) key_row = philox_row(key, grow, head);
+    }
+    if constexpr (READY) {
+      const int q_head = DKV ? head * p.group + h : head;
+      bits = p.bits + (long long)q_head * p.bits_blocks * kBitWords + lane +
+             (DKV ? (quad & 1) * kBlk + (quarter & 1) * 32 : (quarter & 1) * kBlk + (quad & 1) * 32);
+      if (steps > 0) look_ahead();
+    }
     for (int j = 0; j < steps; ++j) {
       const int st = j % kStages, at = C::kBlocks * k + (quarter >> 1);
-      const int e = __shfl_sync(0xffffffffu, at < count ? ulist[at] : 0, 0);
+      int e = next_e;
+      if constexpr (!READY) e = __shfl_sync(0xffffffffu, at < count ? ulist[at] : 0, 0);
       const bool there = at < count;                   // the pair has this block
       const bool mine = (e >> half) & 1;               // it is kept for this warp's rows
       const int blk = e >> 2;
       const uint32_t s_addr = s_base + (j % kSBuf) * C::kCols;
       // words of decisions over the warp's 32 x 32 scores, made for rows of the score matrix: for this thread's own over
-      // its columns (mask: split order, dropout: drop_bit()), or for query `lane` of the block over the warp's keys
+      // its columns (the mask's in split order), or for query `lane` of the block over the warp's keys
       uint32_t mask_w = 0xffffffffu, keep_w = 0xffffffffu;
       if ((MASK || DROP) && mine) {
         const int q_row = DKV ? blk * kBlk + (quarter & 1) * 32 + lane : grow;
@@ -529,12 +625,23 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
           if constexpr (!DKV) mask_w = split_bits32(mask_w);
         }
         if constexpr (DROP) {
-          const int q_head = DKV ? head * p.group + h : head;
-          if constexpr (DKV) key_row = philox_row(key, q_row, q_head);
-          keep_w = philox_bits32<DKV>(key, key_row, t2, word, q_head);
+          if constexpr (READY) {
+            keep_w = next_bits;
+          } else {
+            const int q_head = DKV ? head * p.group + h : head;
+            if constexpr (DKV) key_row = philox_row(key, q_row, q_head);
+            keep_w = philox_bits32(key, key_row, threshold2(p.drop), word, q_head);
+          }
+          if constexpr (DKV) keep_w = fragment_bits(keep_w, lane);
         }
       }
-      if (++k == pairs) { k = 0; ++h; }
+      if (++k == pairs) {
+        k = 0; ++h;
+        if constexpr (DKV && READY) bits += (long long)p.bits_blocks * kBitWords;
+      }
+      if constexpr (READY) {
+        if (j + 1 < steps) look_ahead();
+      }
       if (ok && DKV && !mbar_wait_warp(&full1[st], (j / kStages) & 1)) ok = false;  // the statistics are read here
       if (ok && !mbar_wait_warp(&s_full[j % kSBuf], (j / kSBuf) & 1)) ok = false;
       if (!ok) continue;
@@ -561,7 +668,6 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
           for (int n = 0; n < 4; ++n) {
             const float2 stats = *reinterpret_cast<const float2*>(stat + 8 * n);
             const ColumnMasks m = MASK ? column_masks(mask_w, n, lane) : ColumnMasks{};
-            const ColumnMasks d = DROP ? column_masks(keep_w, n, lane) : ColumnMasks{};
 #pragma unroll
             for (int r = 0; r < 4; ++r) {  // rows lane / 4 + 8 r
               const int i = (r >> 1) * 8 + 2 * n + (r & 1);
@@ -569,7 +675,7 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
               if constexpr (MASK) v = mask_pair(v, m, r);
               prob[i] = v;
               packed[i] = pack2<T>(v.x, v.y);
-              if constexpr (DROP) packed[i] &= packed_mask(d, r);
+              if constexpr (DROP) packed[i] &= packed_mask({keep_w << (2 * r), keep_w << (2 * r + 1)}, n);
             }
           }
         } else {
@@ -615,12 +721,11 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
           for (int n = 0; n < 4; ++n) {
             const float2 stats = *reinterpret_cast<const float2*>(stat + C::kCols + 8 * n);
             const ColumnMasks m = MASK ? column_masks(mask_w, n, lane) : ColumnMasks{};
-            const ColumnMasks d = DROP ? column_masks(keep_w, n, lane) : ColumnMasks{};
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int i = (r >> 1) * 8 + 2 * n + (r & 1);
               float2 v = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-              v = DROP ? fma2(mask_pair(v, d, r), up2, stats) : add2(v, stats);
+              v = DROP ? fma2(mask_pair(v, {keep_w << (2 * r), keep_w << (2 * r + 1)}, n), up2, stats) : add2(v, stats);
               v = mul2(prob[i], v);
               packed[i] = pack2<T>(v.x, v.y);
               // a masked score's probability is zero, and so is its dS whatever stands in V
@@ -632,8 +737,9 @@ __device__ __forceinline__ void bwd_pass(const CUtensorMap& tm_a1, const CUtenso
           for (int i = 0; i < 16; ++i) {
             float2 v = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
             if constexpr (DROP) {
-              v.x = (keep_w >> drop_bit(2 * i)) & 1u ? v.x : 0.f;
-              v.y = (keep_w >> drop_bit(2 * i + 1)) & 1u ? v.y : 0.f;
+              const uint32_t four = keep_w << (i >> 1);  // columns 2 i, 2 i + 1 at the tops of bytes 2 (i & 1) and the next
+              v.x = __uint_as_float(__float_as_uint(v.x) & permute_signs(four, 0, 0x8888u + (i & 1) * 0x2222u));
+              v.y = __uint_as_float(__float_as_uint(v.y) & permute_signs(four, 0, 0x9999u + (i & 1) * 0x2222u));
             }
             v = mul2(prob[i], DROP ? fma2(v, up2, nd) : add2(v, nd));
             packed[i] = pack2<T>(v.x, v.y);
@@ -749,8 +855,19 @@ attn_bwd_kernel(const __grid_constant__ BwdMaps m, const __grid_constant__ BwdPa
                 const __grid_constant__ PassParams q, int kv_blocks) {
   static_assert(BwdCfg<true, D>::kThreads == BwdCfg<false, D>::kThreads, "one launch, one block size");
   const int block = blockIdx.x;
-  if (block < kv_blocks) bwd_pass<true, D, FMT, MASK, DROP, SPLIT>(m.k_tile, m.v_tile, m.q_block, m.do_block, p, kv, block);
-  else bwd_pass<false, D, FMT, MASK, DROP, SPLIT>(m.q_tile, m.do_tile, m.k_block, m.v_block, p, q, block - kv_blocks);
+  auto pass = [&](auto ready) {
+    constexpr bool kReady = decltype(ready)::value;
+    if (block < kv_blocks) bwd_pass<true, D, FMT, MASK, DROP, kReady, SPLIT>(m.k_tile, m.v_tile, m.q_block, m.do_block, p, kv, block);
+    else bwd_pass<false, D, FMT, MASK, DROP, kReady, SPLIT>(m.q_tile, m.do_tile, m.k_block, m.v_block, p, q, block - kv_blocks);
+  };
+  // All of them or none, decided once: a choice in every step cost the steps that have their decisions 40 to 100 us of
+  // 520 (B4 H16 S4096 D64, both passes).  Only the device knows how many blocks there are: `nnz` is a hint.
+  if constexpr (DROP) {
+    if (__ldg(p.blocks) <= p.bits_blocks) pass(std::true_type{});
+    else pass(std::false_type{});
+  } else {
+    pass(std::false_type{});
+  }
 }
 
 int rows_map(CUtensorMap* map, const void* base, int dtype, int D, long long rows, uint32_t box_rows) {
@@ -769,6 +886,7 @@ struct PassPlan {
 };
 constexpr int kMinSteps = 12, kMaxSplit = 16;
 constexpr size_t kMaxPartialBytes = size_t(128) << 20;  // of a pass
+constexpr size_t kMaxBitsBytes = size_t(1) << 30;       // a bit per kept score of every head: as much as Q (D 64) at 16 blocks a row
 
 template <bool DKV, int D>
 PassPlan plan_pass(int heads, int kv_heads, int Nt, int Ns, long long nnz) {
@@ -796,7 +914,7 @@ int present_pitch(int Ns) { return (Ns / kBlk + 1) & ~1; }
 size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
 
 struct Workspace {
-  size_t neg_lse, neg_delta, present, tickets_q, tickets_kv, partial_q, partial_kv, total;
+  size_t neg_lse, neg_delta, present, position, tickets_q, tickets_kv, partial_q, partial_kv, total;  // total: decisions begin
   long long n_tickets;
   PassPlan q, kv;
 };
@@ -809,7 +927,8 @@ Workspace lay_out(int heads, int kv_heads, int Nt, int Ns, long long nnz) {
   w.neg_lse = 0;
   w.neg_delta = w.neg_lse + round16(sizeof(float) * (size_t)heads * Nt);
   w.present = w.neg_delta + round16(sizeof(float) * (size_t)heads * Nt);
-  w.tickets_q = w.present + round16((size_t)(Nt / kBlk) * present_pitch(Ns));
+  w.position = w.present + round16((size_t)(Nt / kBlk) * present_pitch(Ns));
+  w.tickets_q = w.position + round16(sizeof(int32_t) * (size_t)(Nt / kBlk) * present_pitch(Ns));
   w.tickets_kv = w.tickets_q + sizeof(uint32_t) * (size_t)heads * w.q.tiles;
   w.partial_q = w.tickets_q + round16(sizeof(uint32_t) * (size_t)w.n_tickets);
   w.partial_kv = w.partial_q + w.q.partial_bytes;
@@ -830,9 +949,22 @@ int launch_bwd(const AttnArgs& a, BwdParams p, cudaStream_t st) {
   const long long q_rows = (long long)a.heads * a.Nt, k_rows = (long long)a.kv_heads * a.Ns;
   constexpr int kRowsPerBlock = kPrepRows * 2048 / D;
   const long long prep_ctas = (q_rows + kRowsPerBlock - 1) / kRowsPerBlock;
-  attn_bwd_prep_kernel<T, D><<<static_cast<unsigned>(prep_ctas), 256, 0, st>>>(
+  PrepBits make = {};
+  if constexpr (DROP) {
+    make.drop = p.drop;
+    make.heads = a.heads;
+    make.position = reinterpret_cast<int32_t*>(ws + w.position);
+    make.bits = reinterpret_cast<uint32_t*>(ws + w.total);
+    const size_t room = (a.workspace_bytes - w.total) / (sizeof(uint32_t) * kBitWords * (size_t)a.heads);
+    const size_t most = (size_t)(a.Nt / kBlk) * (a.Ns / kBlk);
+    make.blocks = static_cast<int>(room < most ? room : most);
+    p.position = make.position; p.bits = make.bits; p.bits_blocks = make.blocks;
+    const long long items = (long long)make.blocks * a.heads, ctas = (items + 7) / 8;
+    make.ctas = static_cast<int>(ctas < 8 * kNumSMs ? ctas : 8 * kNumSMs);
+  }
+  attn_bwd_prep_kernel<T, D, DROP><<<static_cast<unsigned>(prep_ctas + make.ctas), 256, 0, st>>>(
       static_cast<const T*>(a.O), static_cast<const T*>(a.dO), a.lse, neg_lse, neg_delta, ws + w.present, a.row_ptr, a.idx, q_rows,
-      a.Nt / kBlk, a.Ns / kBlk, p.present_pitch, tickets_q, w.n_tickets);
+      a.Nt / kBlk, a.Ns / kBlk, p.present_pitch, tickets_q, w.n_tickets, make);
   if (int rc = launch_status(); rc != SPARTA_OK) return rc;
   BwdMaps m;
   int rc = rows_map(&m.q_tile, a.Q, a.dtype, D, q_rows, kTileM);
@@ -859,7 +991,8 @@ int launch_bwd(const AttnArgs& a, BwdParams p, cudaStream_t st) {
   const long long q_ctas = a.dQ ? (long long)a.heads * w.q.tiles * w.q.split : 0;
   if (kv_ctas + q_ctas > 0x7fffffffll) return SPARTA_ERR_SHAPE;
   auto launch = [&](auto kern, SmemAttrOnce& attr) {
-    constexpr int kSmem = BwdCfg<true, D>::kSmem > BwdCfg<false, D>::kSmem ? BwdCfg<true, D>::kSmem : BwdCfg<false, D>::kSmem;
+    constexpr int kKv = BwdCfg<true, D>::smem_bytes(DROP), kQ = BwdCfg<false, D>::smem_bytes(DROP), kSmem = kKv > kQ ? kKv : kQ;
+    static_assert((kSmem + 1024) * BwdCfg<true, D>::kCtasPerSM <= 228 * 1024, "shared memory budget");
     if (cudaError_t e = attr.ensure(kern, kSmem); e != cudaSuccess) return static_cast<int>(e);
     kern<<<static_cast<unsigned>(kv_ctas + q_ctas), BwdCfg<true, D>::kThreads, kSmem, st>>>(m, p, kv, q, static_cast<int>(kv_ctas));
     return launch_status();
@@ -884,6 +1017,13 @@ size_t attn_bwd_workspace(int heads, int kv_heads, int Nt, int Ns, int D, long l
   return D == 64 ? lay_out<64>(heads, kv_heads, Nt, Ns, nnz).total : lay_out<128>(heads, kv_heads, Nt, Ns, nnz).total;
 }
 
+// Room for the dropout decisions of `nnz` blocks for every head, up to kMaxBitsBytes.
+size_t attn_bwd_dropout_workspace(int heads, long long nnz) {
+  const size_t block = sizeof(uint32_t) * kBitWords * (size_t)heads;
+  const size_t fit = kMaxBitsBytes / block;
+  return block * ((size_t)nnz < fit ? (size_t)nnz : fit);
+}
+
 int attn_bwd_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* status, cudaStream_t st) {
   if (a.Ns / kBlk > kMaxBlocks || a.Nt / kBlk > kMaxBlocks) return SPARTA_ERR_UNSUPPORTED;
   BwdParams p = {};
@@ -892,6 +1032,7 @@ int attn_bwd_launch(const AttnArgs& a, const DropoutParams& drop, int32_t* statu
   p.scale = a.scale; p.scale_log2 = a.scale * 1.4426950408889634f;
   p.status = status;
   p.drop = drop;
+  p.blocks = a.row_ptr + a.Nt / kBlk;
   if (a.D == 64) return a.dtype == SPARTA_F16 ? launch_variant<64, 0>(a, p, st) : launch_variant<64, 1>(a, p, st);
   return a.dtype == SPARTA_F16 ? launch_variant<128, 0>(a, p, st) : launch_variant<128, 1>(a, p, st);
 }

@@ -557,6 +557,7 @@ int train_args(const sparta_attn_train_args* h, AttnArgs* a, DropoutParams* drop
   a->kv_heads = h->kv_heads;
   a->dO = h->dO; a->dQ = h->dQ; a->dK = h->dK; a->dV = h->dV;
   a->workspace = h->workspace;
+  a->workspace_bytes = h->workspace_bytes;
   a->nnz = h->nnz_hint;
   if (h->nnz_hint < 0) return SPARTA_ERR_BAD_ARG;
   if (!aligned(h->lse, 4) || (h->rng && !aligned(h->rng, 8))) return SPARTA_ERR_ALIGN;
@@ -603,6 +604,10 @@ extern "C" int sparta_attn_train_fwd(const sparta_attn_train_args* h_args, void*
 extern "C" size_t sparta_attn_train_bwd_workspace_bytes(int heads, int kv_heads, int Nt, int Ns, int D, int64_t nnz_hint) {
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || Nt <= 0 || Ns <= 0 || (D != 64 && D != 128) || nnz_hint < 0) return 0;
   return attn_bwd_workspace(heads, kv_heads, Nt, Ns, D, nnz_hint);
+}
+
+extern "C" size_t sparta_attn_train_bwd_dropout_bytes(int heads, int64_t nnz_hint) {
+  return heads <= 0 || nnz_hint <= 0 ? 0 : attn_bwd_dropout_workspace(heads, nnz_hint);
 }
 
 extern "C" int sparta_attn_train_bwd(const sparta_attn_train_args* h_args, void* stream) {

@@ -5,7 +5,7 @@
 //   counter = (c / 8, r, b, call)   key = seed   ->   128 bits = eight 16-bit values, the one of column c at place c % 8
 //   keep    <=>   value >= threshold,   threshold = round(65536 p)
 // so a dense tensor, block values in any block size, and the fused attention kernels (forward, and the backward
-// passes that hold the scores one way round or the other) all drop the same positions, and nothing is stored.  Eight
+// passes that hold the scores one way round or the other) all drop the same positions, and nothing is kept between them.  Eight
 // decisions per call of the generator: 16 bits resolve p to 1 / 65536, and the scale 65536 / (65536 - threshold) is
 // that of the rounded probability, so the expectation is exact.
 #pragma once

@@ -330,7 +330,8 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
       if (q.numel() > 0) {
         const c10::cuda::CUDAGuard guard(q.device());
         sparta_attn_train_args a = attention_args(q, k, v, out, s[4], s[5], s[6], optional_of(s[7]), s[8], optional_of(s[9]), c);
-        const size_t bytes = sparta_attn_train_bwd_workspace_bytes(a.heads, a.kv_heads, a.Nt, a.Ns, a.D, a.nnz_hint);
+        size_t bytes = sparta_attn_train_bwd_workspace_bytes(a.heads, a.kv_heads, a.Nt, a.Ns, a.D, a.nnz_hint);
+        if (c.p > 0) bytes += sparta_attn_train_bwd_dropout_bytes(a.heads, a.nnz_hint);
         const Tensor workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
         a.dO = grad.const_data_ptr();
         a.dQ = want_q ? dq.data_ptr() : nullptr;

@@ -53,3 +53,11 @@ def test_refusals():
     sizes = [L.sparta_attn_train_bwd_workspace_bytes(*long, n) for n in (0, 2000, 20000, 1 << 20)]
     assert sizes[0] < sizes[1] and sizes[0] == sizes[3] and max(sizes) <= sizes[0] + (256 << 20)
     assert bwd(args(workspace_bytes=need, nnz_hint=0, workspace=None), None) == -4
+
+
+def test_room_for_dropout_decisions():
+    f = _lib.lib().sparta_attn_train_bwd_dropout_bytes
+    assert f(16, 100) == 16 * 100 * 64 * 64 // 8  # a bit per kept score
+    assert f(0, 100) == 0 and f(-1, 100) == 0 and f(16, 0) == 0 and f(16, -5) == 0
+    # a bound, and whole blocks of every head below it
+    assert f(16, 1 << 40) <= 1 << 30 and f(16, 1 << 40) % (16 * 512) == 0 and f(1 << 30, 1) == 0

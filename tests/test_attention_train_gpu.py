@@ -10,6 +10,7 @@ from oracle import oracle as masks
 from sparta_b200 import _lib
 from sparta_b200.nn import RotaryEmbedding, SparseAttention
 from sparta_b200.specializer.operators.rotary import rotary_frequencies
+from sparta_b200.tesa import get_bcs_function
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float16, torch.bfloat16]
@@ -532,3 +533,41 @@ def test_long_sequences_with_global_tokens():
         for name, x, y in zip(('out', 'dq', 'dk', 'dv'), (got[0][h], got[1][h], got[2][kv], got[3][kv]), want):
             rel = ((x.detach().double() - y).norm() / y.norm()).item()
             assert rel <= 4 * torch.finfo(torch.bfloat16).eps / 2, f'{name} of head {kv}: {rel}'
+
+
+@pytest.mark.parametrize('elements', [False, True])
+@pytest.mark.parametrize('dim', [64, 128])
+def test_dropout_decisions_made_once_or_in_every_pass(dim, elements):
+    """Room for the decisions of all kept blocks, of all but one, of none: the same gradients bit for bit, and nothing
+    is written behind the workspace."""
+    heads, kv_heads, nt, ns = 6, 2, 320, 448
+    q, k, v, do = (t.cuda() for t in inputs(torch.float16, heads, kv_heads, nt, ns, dim))
+    mask = block_mask(nt, ns, 0.5, elements=elements).cuda()
+    idx = get_bcs_function(64, 64, True, False).build_indexes(mask)
+    L, n, numbers = _lib.lib(), idx.block_nnz, rng(5, 9)
+    out, lse = torch.empty_like(q), torch.empty((heads, nt), device='cuda')
+    status = torch.zeros(4, dtype=torch.int32, device='cuda')
+    stream = torch.cuda.current_stream().cuda_stream
+    a = _lib.AttnTrainArgs(Q=q.data_ptr(), K=k.data_ptr(), V=v.data_ptr(), O=out.data_ptr(), lse=lse.data_ptr(), dO=do.data_ptr(),
+                           row_ptr=idx.row_ptr.data_ptr(), bcsr_idx=idx.bcsr_buf.data_ptr(), mask=mask.data_ptr() if elements else None,
+                           rng=numbers.data_ptr(), status=status.data_ptr(), dropout=0.25, scale=dim ** -0.5, heads=heads,
+                           kv_heads=kv_heads, Nt=nt, Ns=ns, D=dim, BLK=64, dtype=_lib.F16)
+    assert L.sparta_attn_train_fwd(a, stream) == 0
+    base = L.sparta_attn_train_bwd_workspace_bytes(heads, kv_heads, nt, ns, dim, 0)
+    every = L.sparta_attn_train_bwd_dropout_bytes(heads, n)
+    assert every == heads * n * 512
+    results = []
+    for extra in (0, 1, every - 512, every - 1, every, every + 4096, 2 * heads * nt * ns):
+        room = torch.full((base + extra + 256,), 0xa5, dtype=torch.uint8, device='cuda')
+        grads = [torch.full_like(t, math.nan) for t in (q, k, v)]
+        a.workspace, a.workspace_bytes = room.data_ptr(), base + extra
+        a.dQ, a.dK, a.dV = (t.data_ptr() for t in grads)
+        assert L.sparta_attn_train_bwd(a, stream) == 0
+        assert bool((room[base + extra:] == 0xa5).all()) and not status.any()
+        results.append(grads)
+    for grads in results[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(grads, results[0]))
+    keep = oracle.dropout_keep(5, 9, heads, nt, ns, 0.25)
+    want, bounds = want_and_bounds(q.cpu(), k.cpu(), v.cpu(), do.cpu(), mask.cpu(), keep, oracle.dropout_scale(0.25))
+    for got, w, e in zip([out] + results[0], want, bounds):
+        assert bool(((got.double().cpu() - w).abs() <= e).all())
