@@ -46,7 +46,7 @@
 // Masks and dropout are words of 32 decisions per row of the score matrix (query): in the dQ pass each thread's own, in
 // the dK, dV pass each lane has one and the threads fetch those of their eight columns from the lanes that have them.
 // Dropout decisions are made once, by the first kernel, for both passes, if the workspace has room (B4 H16 S4096 D64,
-// p = 0.1: 716 us with the generator in the steps of both; 621 us now, of which 95 the first kernel, 520 the passes).
+// p = 0.1: 716 us with the generator in the steps of both; 610 us now, of which 94 the first kernel, 515 the passes).
 // The forward pass it belongs to: SparseAttention.forward (sparta/specializer/operators/sparse_attention.py:76-80),
 // whose gradients the reference takes through its three operators.
 #include <type_traits>
@@ -268,7 +268,7 @@ attn_bwd_prep_kernel(const T* __restrict__ O, const T* __restrict__ dO, const fl
       const int c = __ldg(idx + e) & 0xffff;
       if (c < nbc) {  // index arrays come from the caller: never index shared memory with them unchecked
         kept[c] = 1;
-        if constexpr (DROP) make.position[(long long)r * pitch + c] = e;
+        if constexpr (DROP) make.position[(long long)r * pitch + c] = max(0, min(e, make.blocks - 1));  // (nor the workspace)
       }
     }
     __syncthreads();
